@@ -51,6 +51,22 @@ int encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
   return r == CUDA_SUCCESS ? FB_OK : FB_ERR_DRIVER;
 }
 
+int encode_u8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols, uint32_t box_rows) {
+  std::call_once(g_encode_once, load_encoder);
+  if (g_encode == nullptr) return FB_ERR_DRIVER;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return FB_ERR_ARG;
+  if (rows == 0 || rows > (1ull << 32) || (cols != 64 && cols != 128)) return FB_ERR_SHAPE;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols};
+  cuuint32_t box[2] = {cols, box_rows};
+  cuuint32_t elem_strides[2] = {1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                        elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FB_OK : FB_ERR_DRIVER;
+}
+
 int sm_count() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;

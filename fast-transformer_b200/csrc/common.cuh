@@ -266,6 +266,9 @@ namespace fb {
 // `pitch_elems`, box {box_cols, box_rows}, 128-byte swizzle. Returns FB_OK or an error.
 int encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                    uint64_t pitch_elems, uint32_t box_cols, uint32_t box_rows, bool swizzle128);
+// The same over a dense [rows, cols] byte matrix, cols 64 or 128, boxes of whole rows swizzled by
+// their length (64- or 128-byte swizzle).
+int encode_u8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols, uint32_t box_rows);
 int sm_count();
 int check_launch();
 // Device address of the error word on the current device (kernels take it as a parameter).

@@ -46,6 +46,18 @@ _SIGNATURES = {
     "fb_qk_norm_rope_append": (_c_int, [_vp, _c_int, _vp, _vp, _c_float, _c_float, _vp, _vp, _vp, _vp,
                                         _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                         _c_int, _c_int, _vp]),
+    "fb_qk_norm_rope_append_q8": (_c_int, [_vp, _c_int, _vp, _vp, _c_float, _c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                           _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                           _c_int, _c_int, _vp]),
+    "fb_spec_relocate_q8": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
+    "fb_attention_q8_workspace": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "fb_attention_q8": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int,
+                                 _c_int, _c_int, _c_int, _c_int, _c_float, _vp]),
+    "fb_w4_packed_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "fb_w4_scale_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "fb_w4_pack": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "fb_w4_dequantize": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "fb_linear_w4": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
     "fb_rmsnorm": (_c_int, [_vp, _c_i64, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
     "fb_add_rmsnorm": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
     "fb_embed_rmsnorm": (_c_int, [_vp, _vp, _c_i64, _vp, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
@@ -99,7 +111,7 @@ def exported_names():
 
 
 #: Kernels each launching entry point enqueues (fb_argmax runs two stages).
-_KERNELS_PER_CALL = {"fb_argmax": 2}
+_KERNELS_PER_CALL = {"fb_argmax": 2, "fb_attention_q8": 2}
 _NON_LAUNCHING = {"fb_device_error"}
 #: Running count of libfastb200 kernels enqueued (or recorded into a graph) by this process.
 launches = 0
@@ -118,6 +130,18 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def launch(name, device, *args):
+    """Calls entry point ``name`` with ``args`` and the current stream of ``device``, with that device
+    current for the call (launch shapes and the error word go by the current device)."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    check(status, name)
+
+
 def ptr(tensor):
     return ctypes.c_void_p(tensor.data_ptr()) if tensor is not None else None
 
@@ -127,6 +151,15 @@ def device_error():
     flags = ctypes.c_uint(0)
     check(lib.fb_device_error(ctypes.byref(flags)), "fb_device_error")
     return flags.value
+
+
+def require_device(device, *tensors):
+    """Every tensor on the one CUDA device ``device``."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"libfastb200 kernels take tensors of one device: {t.device} and {device}")
+    if device.type != "cuda":
+        raise ValueError("libfastb200 kernels take CUDA tensors only (no CPU fallback)")
 
 
 def require_cuda(*tensors):

@@ -7,6 +7,9 @@ contributes; the result is a new [B,1,Hq,D] tensor. Additionally ``position`` ma
 one entry per row ([B]) for ragged batches. The kernels are fb_decode_attention (TMA +
 mma.sync partials over a balanced persistent split) and fb_decode_attention_combine
 (log-sum-exp merge), launched on the current stream, so CUDA-graph capture records them.
+
+``decode_attention_q8`` and ``block_attention_q8`` are the same calls over an 8-bit cache
+(kernels.quant.QuantCache; fb_attention_q8, no counterpart in the reference).
 """
 
 import torch
@@ -114,3 +117,40 @@ def block_attention(query, key, value, position, scale, chain, splits=None):
     if splits > 1:
         _native.launches += 1  # the split merge
     return out
+
+
+def _attend_q8(query, cache, position, per_row, chain, tokens, q_heads, shape, scale):
+    device = query.device
+    _native.require_device(device, cache.keys, position, chain)
+    assert query.dtype == torch.bfloat16 and query.is_contiguous()
+    assert position.dtype == torch.int64 and position.is_contiguous()
+    out = torch.empty(shape, device=device, dtype=torch.bfloat16)
+    need = cache.workspace_bytes(tokens, q_heads)
+    if need == 0:
+        raise ValueError(f"attention over {cache.batch} x {cache.kv_heads} x {cache.capacity} slots is too large")
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _native.launch("fb_attention_q8", device, query.data_ptr(), cache.keys.data_ptr(), cache.values.data_ptr(),
+                   cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), position.data_ptr(), per_row,
+                   chain.data_ptr() if chain is not None else None, out.data_ptr(), workspace.data_ptr(), need,
+                   cache.batch, tokens, q_heads, cache.kv_heads, cache.dim, cache.capacity, cache.block, scale)
+    return out
+
+
+def decode_attention_q8(query, cache, position, scale):
+    """``decode_attention`` over a ``QuantCache``: Q [B,Hq,1,D] -> [B,1,Hq,D]; ``position`` int64 [1]
+    or [B]. A row at position -1 (or below) holds nothing and gives zeros."""
+    batch, q_heads, tokens, dim = query.shape
+    assert tokens == 1 and batch == cache.batch and dim == cache.dim and q_heads % cache.kv_heads == 0
+    assert position.shape == (1,) or position.shape == (batch,)
+    return _attend_q8(query, cache, position, 1 if position.shape[0] > 1 else 0, None, 1, q_heads,
+                      (batch, 1, q_heads, dim), float(scale))
+
+
+def block_attention_q8(query, cache, position, scale, chain):
+    """``block_attention`` over a ``QuantCache``: token-major Q [B,T,Hq,D], position and chain int64
+    [B] -> [B,T,Hq,D]. The block's own keys and values must already be in the cache."""
+    batch, tokens, q_heads, dim = query.shape
+    assert 0 < tokens <= cache.capacity and batch == cache.batch and dim == cache.dim
+    assert q_heads % cache.kv_heads == 0 and position.shape == (batch,)
+    assert chain.shape == (batch,) and chain.dtype == torch.int64 and chain.is_contiguous()
+    return _attend_q8(query, cache, position, 1, chain, tokens, q_heads, (batch, tokens, q_heads, dim), float(scale))

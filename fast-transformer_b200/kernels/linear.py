@@ -11,6 +11,10 @@ stay on cuBLAS through ``F.linear``, exactly as the reference routes them (linea
 ``keep_native`` is the reference's hook for leaving a shape on cuBLAS without tuning it
 (linear.py:484-486); the B200 kernels choose their launch shape by a fixed rule (no timed
 search), so it only records the request.
+
+``linear``, ``swiglu_linear`` and ``project`` also take 4-bit weights (kernels.quant.Weight4):
+fb_linear_w4 up to MAX_ROWS rows, one launch whose result is finished (never a ``Split``); more
+rows go to cuBLAS on the weights expanded to BF16 for the call. The reference has no such form.
 """
 
 import torch
@@ -19,6 +23,7 @@ from torch.nn import functional as F
 from kernels import _native
 from kernels._native import check, lib, ptr, stream
 from kernels.merged import Split
+from kernels.quant import Weight4
 
 #: Rows the skinny kernel takes (x is staged as 16/32/64-row slabs).
 MAX_ROWS = 64
@@ -55,7 +60,9 @@ def supported(rows, weight):
 
 def project(flat, weight, epilogue=BF16_OUT, splits=None):
     """fb_linear on [M,K] x [N,K]: BF16 [M,N], FP32 [M,N], SwiGLU BF16 [M,N/2] or FP32 split
-    partials [S,M,N]."""
+    partials [S,M,N] (4-bit weights: S is 1)."""
+    if isinstance(weight, Weight4):
+        return _project4(flat, weight, epilogue)
     m, k = flat.shape
     n = weight.shape[0]
     if splits is None:
@@ -70,8 +77,48 @@ def project(flat, weight, epilogue=BF16_OUT, splits=None):
     return out
 
 
+def _project4(flat, weight, epilogue):
+    """fb_linear_w4 on [M,K]: the outputs of ``project``."""
+    m, k = flat.shape
+    n = weight.shape[0]
+    if k != weight.shape[1] or flat.dtype != torch.bfloat16 or not 0 < m <= MAX_ROWS:
+        raise ValueError(f"4-bit weights {tuple(weight.shape)} take 1 to {MAX_ROWS} BF16 rows of their width, not "
+                         f"{flat.dtype} {tuple(flat.shape)}")
+    device = flat.device
+    _native.require_device(device, weight.packed)
+    if epilogue == SWIGLU_OUT:
+        if n % 128:
+            raise ValueError(f"SwiGLU weights are 64-row gate/up blocks: {n} rows are not a multiple of 128")
+        out = torch.empty((m, n // 2), device=device, dtype=torch.bfloat16)
+    elif epilogue == SPLITS_OUT:
+        out = torch.empty((1, m, n), device=device, dtype=torch.float32)
+    else:
+        out = torch.empty((m, n), device=device, dtype=torch.float32 if epilogue == FP32_OUT else torch.bfloat16)
+    if flat.data_ptr() % 16:
+        flat = flat.clone()
+    _native.launch("fb_linear_w4", device, flat.data_ptr(), weight.packed.data_ptr(), weight.scales.data_ptr(),
+                   out.data_ptr(), m, n, k, weight.group, FP32_OUT if epilogue == SPLITS_OUT else epilogue)
+    return out
+
+
+def _linear4(x, weight):
+    n, k = weight.shape
+    if x.shape[-1] != k or x.dtype != torch.bfloat16:
+        raise ValueError(f"4-bit weights {tuple(weight.shape)} take BF16 [..., {k}], not {x.dtype} {tuple(x.shape)}")
+    rows = x.numel() // k
+    if rows == 0:
+        return x.new_empty((*x.shape[:-1], n))
+    if rows > MAX_ROWS:
+        _native.require_device(weight.device, x)
+        return F.linear(x, weight.dequantized())
+    return _project4(x.reshape(rows, k).contiguous(), weight, BF16_OUT).view(*x.shape[:-1], n)
+
+
 def linear(x, weight, split_ok=False):
-    """x @ weight.T in BF16. With ``split_ok`` the result may be a ``Split`` for a consumer kernel."""
+    """x @ weight.T in BF16. With ``split_ok`` the result may be a ``Split`` for a consumer kernel.
+    ``weight``: a BF16 [N, K] tensor or a ``Weight4``."""
+    if isinstance(weight, Weight4):
+        return _linear4(x, weight)
     rows = x.numel() // x.shape[-1]
     if x.dtype != torch.bfloat16 or not weight.is_contiguous() or not supported(rows, weight):
         return F.linear(x, weight)
@@ -96,6 +143,8 @@ def swiglu_linear(x, gate_up_blocked):
     rows = x.numel() // x.shape[-1]
     flat = x.reshape(rows, x.shape[-1]).contiguous()
     n, k = gate_up_blocked.shape
+    if isinstance(gate_up_blocked, Weight4):  # finished in the projection's launch
+        return _project4(flat, gate_up_blocked, SWIGLU_OUT).view(*x.shape[:-1], n // 2)
     splits = splits_for(rows, n, k, x.device)
     if splits == 1:
         return project(flat, gate_up_blocked, SWIGLU_OUT, splits).reshape(*x.shape[:-1], n // 2)

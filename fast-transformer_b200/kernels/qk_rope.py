@@ -2,7 +2,8 @@
 
 Drop-in for engine/kernels/qk_rope.py:87-129 (same signature, asserts and return value):
 one launch of fb_qk_norm_rope_append writes token-major Q and appends K (normed, rotated)
-and V (copied) at each token's cache slot.
+and V (copied) at each token's cache slot. ``qk_rope_cache_q8`` is the same call on an 8-bit
+cache (kernels.quant.QuantCache; fb_qk_norm_rope_append_q8, no counterpart in the reference).
 """
 
 import torch
@@ -48,4 +49,44 @@ def qk_rope_cache(packed, q_norm, k_norm, cos, sin, position, keys, values, q_he
         ptr(position), ptr(phases) if table else None, ptr(query), ptr(keys), ptr(values),
         batch, tokens, q_heads, kv_heads, dim, capacity, mode, 1 if table else 0, stream(),
     ), "fb_qk_norm_rope_append")
+    return query.transpose(1, 2)
+
+
+def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, cache, q_heads, prefill=False, rows=False, phases=None,
+                     table=False):
+    """``qk_rope_cache`` into a ``QuantCache``: norm and RoPE in fp32, Q rounded once to BF16, K and V
+    once to e4m3 under their block's scale. ``table`` (decode mode) or ``phases`` (rows mode): cos
+    and sin are whole tables of at least ``cache.capacity`` rows, read at the device-side position.
+    Rows at a negative position get nothing appended."""
+    split = isinstance(packed, Split)
+    data, splits, _, shape = source(packed)
+    batch, kv_heads, capacity, dim = cache.batch, cache.kv_heads, cache.capacity, cache.dim
+    tokens = shape[1]
+    device = data.device
+    assert data.dtype == (torch.float32 if split else torch.bfloat16) and data.is_contiguous()
+    assert shape == (batch, tokens, (q_heads + 2 * kv_heads) * dim) and q_heads > 0
+    assert 0 < tokens <= capacity
+    assert not (rows and prefill) and not (table and (rows or prefill))
+    if phases is not None:
+        assert rows and phases.shape == (batch, tokens) and phases.is_contiguous() and phases.dtype == torch.int64
+    whole = table or phases is not None
+    assert cos.dtype == sin.dtype == torch.bfloat16 and cos.is_contiguous() and sin.is_contiguous()
+    if whole:
+        assert cos.shape == sin.shape and cos.shape[-1] == dim and cos.numel() >= capacity * dim
+    else:
+        assert cos.numel() == sin.numel() == (batch if rows else 1) * tokens * dim
+    assert position.shape == ((tokens,) if prefill else (batch,) if rows else (1,))
+    assert position.dtype == torch.int64 and position.is_contiguous()
+    q_weight, k_weight = q_norm.weight, k_norm.weight
+    assert q_weight.dtype == k_weight.dtype == torch.bfloat16 and q_weight.numel() == k_weight.numel() == dim
+    assert q_weight.is_contiguous() and k_weight.is_contiguous()
+    _native.require_device(device, cache.keys, cos, sin, position, phases, q_weight, k_weight)
+    query = torch.empty((batch, tokens, q_heads, dim), device=device, dtype=torch.bfloat16)
+    _native.launch(
+        "fb_qk_norm_rope_append_q8", device, data.data_ptr(), splits if split else 0, q_weight.data_ptr(),
+        k_weight.data_ptr(), q_norm.variance_epsilon, k_norm.variance_epsilon, cos.data_ptr(), sin.data_ptr(),
+        position.data_ptr(), phases.data_ptr() if phases is not None else None, query.data_ptr(),
+        cache.keys.data_ptr(), cache.values.data_ptr(), cache.key_scales.data_ptr(), cache.value_scales.data_ptr(),
+        batch, tokens, q_heads, kv_heads, dim, capacity, cache.block, 1 if prefill else 2 if rows else 0,
+        1 if whole else 0)
     return query.transpose(1, 2)

@@ -3,6 +3,7 @@
 Drop-in for engine/kernels/spec.py: ``propose`` (:106-124), ``within_margin`` (:154-166),
 ``settle`` (:227-240) and ``relocate`` (:262-270), with the same signatures, asserts and
 in-place effects, each one fb_spec_* launch of libfastb200 on the current stream.
+``relocate_q8`` is the KV move in an 8-bit store (no counterpart in the reference).
 """
 
 import torch
@@ -63,3 +64,19 @@ def relocate(store, move_from, move_to):
     _native.require_cuda(store, move_from, move_to)
     check(lib.fb_spec_relocate(ptr(store), planes * layers, batch, kv_heads, capacity, dim, ptr(move_from),
                                ptr(move_to), stream()), "fb_spec_relocate")
+
+
+def relocate_q8(store, scales, block, move_from, move_to):
+    """``relocate`` in an 8-bit store: e4m3 codes [2, L, B, Hkv, C, D], fp32 scales [2, L, B, Hkv,
+    ceil(C / block)] (kernels.quant). ``move_to`` becomes its block's newest slot: its block's
+    scale follows the append's rule."""
+    planes, layers, batch, kv_heads, capacity, dim = store.shape
+    assert store.dtype == torch.float8_e4m3fn and store.is_contiguous() and planes == 2
+    assert dim in (64, 128) and block in (16, 32, 64)
+    assert scales.dtype == torch.float32 and scales.is_contiguous()
+    assert scales.shape == (planes, layers, batch, kv_heads, -(-capacity // block))
+    assert move_from.shape == move_to.shape == (batch,) and move_from.dtype == move_to.dtype == torch.int64
+    assert move_from.is_contiguous() and move_to.is_contiguous()
+    _native.require_device(store.device, scales, move_from, move_to)
+    _native.launch("fb_spec_relocate_q8", store.device, store.data_ptr(), scales.data_ptr(), planes * layers, batch,
+                   kv_heads, capacity, dim, block, move_from.data_ptr(), move_to.data_ptr())
