@@ -13,26 +13,29 @@
 // can neither overflow nor wash out P's f16 range, while the denominator sums 2^(s - m) in
 // fp32. Q is scaled by a power of two to f16's range (exact for any bf16 row).
 //
-// Bound by the bytes of codes; 148 persistent CTAs cut the 128-slot tiles of all (row, KV head,
-// member group) units into equal contiguous slices, so ragged rows balance. A run of tiles that
-// covers its unit writes the output; others leave (O, M, m, l) partials, merged in CTA order by
-// a second launch (no counters, no atomics: two calls never share state).
-//  * Warp 8 is the producer: one lane issues a TMA load per K and V tile (128 rows of D bytes,
-//    swizzled by the row's length), 16 lanes copy the tile's per-slice scales with cp.async; both
-//    complete on the stage's mbarrier.
-//  * Warps 0-7 take 16 slots each: S^T[16 x 8 NG] = K Q^T, lazy pivot (it moves only when a score
-//    passes it by more than 8, one vote), O^T += V^T P^T.
-//  * Members = the T * G query heads that share a KV head, in groups of 8 NG columns.
+// Bound by the bytes of codes. Members = the T * G query heads that share a KV head, in groups of
+// 8 NG columns; a unit = (row, KV head, member group); its tiles are 64 slots of K and V. A CTA is
+// a producer warp (one lane issues a TMA load per K and V tile, 8 lanes copy the tile's scales
+// with cp.async; both complete on the stage's mbarrier) and four consumer warps of 16 slots each:
+// S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a score passes it by more than 8, one
+// vote), O^T += V^T P^T. Two CTAs share an SM, so that one streams while the other starts or ends.
+//  * Few units: a cluster of C CTAs per unit (interleaved tiles), merged by pushing each
+//    partial to its output's owner through distributed shared memory: one launch, no workspace.
+//  * Many units: a persistent grid cuts the tiles of all units into equal contiguous slices, so
+//    ragged rows balance. A run of tiles that covers its unit writes the output; others leave
+//    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
+//    calls share nothing.
 #include "q8.cuh"
 
 namespace fb {
 namespace attn8 {
 
-constexpr int kTile = 128;
-constexpr int kWarps = 8;  // 16 slots each
+constexpr int kWarps = 4;  // consumers: 16 slots of a tile each
+constexpr int kTile = 16 * kWarps;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kMaxBatch = 1024;
 constexpr int kScales = 2 * kWarps;  // per stage: K and V scale of each 16-slot slice
+constexpr int kMaxCluster = 16;      // above 8: the non-portable cluster size attribute
 constexpr float kSlack = 8.f;        // log2 a score may pass the pivot by: p <= 2^8, exact enough in f16
 
 struct Params {
@@ -59,7 +62,7 @@ __device__ __forceinline__ int row_length(const Params& p, int b) {
   if (n < 0) return 0;
   return n > p.capacity - p.tokens ? p.capacity : static_cast<int>(n) + p.tokens;
 }
-__device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+__host__ __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
 __device__ __forceinline__ long long slice_start(long long total, int i, int ctas) { return total * i / ctas; }
 __device__ __forceinline__ int slice_owner(long long total, long long tile, int ctas) {
   return static_cast<int>(((tile + 1) * ctas - 1) / total);
@@ -101,59 +104,70 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) {
   return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4);
 }
 
-template <int D>
+template <int D, int NG>
 struct Smem {
   static constexpr int kTileBytes = kTile * D;
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kScaleBytes = kStages * kScales * 4;
-  static constexpr int kRedO = kWarps * D * 8 * 4;      // one 8-column group of every warp
-  static constexpr int kRedStats = kWarps * 32 * 3 * 4;  // M, m, l of up to 32 columns
+  static constexpr int kQueryPitch = D * 2 + 32;  // f16 query rows, padded against bank conflicts
+  static constexpr int kQuery = NG * 8 * kQueryPitch;
+  static constexpr int kRedO = kWarps * D * 8 * 4;           // one 8-column group of every warp
+  static constexpr int kRedStats = kWarps * NG * 8 * 3 * 4;  // M, m, l
+  // persistent form: tile counts before each row; cluster form: O received as an owner
+  // ([rank][chunk], C * ceil(n / C) <= n + C - 1 values) and every rank's M, m, l
   static constexpr int kCum = ((kMaxBatch + 1) * 4 + 15) & ~15;
+  static constexpr int kRecvO = (NG * 8 * D + kMaxCluster) * 4;
+  static constexpr int kRecvStats = kMaxCluster * NG * 8 * 3 * 4;
+  static constexpr int kShared = kCum > kRecvO + kRecvStats ? kCum : kRecvO + kRecvStats;
   static constexpr int kBars = 2 * kStages * 8;
-  static constexpr int kTotal = 1024 + kRing + kScaleBytes + kRedO + kRedStats + kCum + kBars + 32;
+  static constexpr int kTotal = 1024 + kRing + kScaleBytes + kQuery + kRedO + kRedStats + kShared + kBars + 32;
+  static_assert((kScaleBytes + kQuery + kRedO + kRedStats + kShared) % 16 == 0, "mbarrier alignment");
+
+  uint8_t* ring;
+  float* scales;
+  uint8_t* query;
+  float* red_o;
+  float* red_stats;
+  int* cum;
+  float* recv_o;
+  float* recv_stats;
+  uint64_t* full;
+  uint64_t* empty;
+  volatile int* misc;  // [0..2]: first row, unit, tile; [3]: abort
+
+  __device__ explicit Smem(uint8_t* raw) {
+    ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    scales = reinterpret_cast<float*>(ring + kRing);
+    query = ring + kRing + kScaleBytes;
+    red_o = reinterpret_cast<float*>(query + kQuery);
+    red_stats = red_o + kRedO / 4;
+    cum = reinterpret_cast<int*>(red_stats + kRedStats / 4);
+    recv_o = reinterpret_cast<float*>(cum);
+    recv_stats = recv_o + kRecvO / 4;
+    full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(cum) + kShared);
+    empty = full + kStages;
+    misc = reinterpret_cast<volatile int*>(empty + kStages);
+  }
 };
 
-// A consumer warp's state on one unit.
+// A consumer warp's state on one unit. At one column group the query's B fragments stay in
+// registers; with more they are read from shared memory for every tile (the accumulators need
+// the registers).
 template <int D, int NG>
 struct State {
-  uint32_t q[NG][D / 16][2];  // B fragments: member column lane / 4 of each group
+  uint32_t q[NG == 1 ? D / 16 : 1][2];
   float o[NG][D / 16][4];
   float m[NG][2], M[NG][2], l[NG][2];  // columns 2c, 2c + 1
   float qs[NG][2];                     // score multiplier of those columns: 2^e scale log2(e)
 };
 
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32) : "memory"); }
+
 template <int D, int NG>
-__device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, int b, int h, int chunk, int lane) {
-  const int g = lane >> 2, c = lane & 3;
+__device__ __forceinline__ void clear(State<D, NG>& a) {
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
-    const int member = chunk * p.width + n * 8 + g;
-    const bool live = n * 8 + g < p.width && member < p.members;
-    const int t = live ? member / p.groups : 0;
-    const int head = h * p.groups + (live ? member % p.groups : 0);
-    const __nv_bfloat16* row = p.q + ((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D;
-    float x[D / 16][4];
-    float top = 0.f;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const uint2 w = live ? *reinterpret_cast<const uint2*>(row + k * 16 + 4 * c) : make_uint2(0u, 0u);
-      x[k][0] = bf16_lo(w.x), x[k][1] = bf16_hi(w.x), x[k][2] = bf16_lo(w.y), x[k][3] = bf16_hi(w.y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[k][e]));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the row's largest magnitude to [2^14, 2^15): every value keeps its bits unless it is 2^-28 of it
-    const int up = top > 0.f && top < INFINITY ? 14 - ilogbf(top) : 0;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      a.q[n][k][0] = pack_f16x2(ldexpf(x[k][0], up), ldexpf(x[k][1], up));
-      a.q[n][k][1] = pack_f16x2(ldexpf(x[k][2], up), ldexpf(x[k][3], up));
-    }
-    const float mine = ldexpf(p.scale_log2, -up);  // of column g; this thread's scores are 2c and 2c + 1
-    a.qs[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
-    a.qs[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) a.o[n][k][0] = a.o[n][k][1] = a.o[n][k][2] = a.o[n][k][3] = 0.f;
 #pragma unroll
@@ -162,6 +176,69 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, int
       a.l[n][e] = 0.f;
     }
   }
+}
+
+// The unit's queries as f16 B fragments: lane (g, c) holds dims 16 k + 4 c .. + 3 of member column
+// g, the order in which K's fragments hold the dims. The row's largest magnitude is scaled to
+// [2^14, 2^15): every value keeps its bits unless it is below 2^-28 of it.
+template <int D, int NG>
+__device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uint8_t* query, int b, int h, int chunk,
+                                           int warp, int lane) {
+  using S = Smem<D, NG>;
+  const int g = lane >> 2, c = lane & 3;
+  if (NG > 1) consumers_sync();  // the last unit's queries have been read
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    if (NG > 1 && n % kWarps != warp) continue;  // with shared queries each warp converts its groups
+    const int member = chunk * p.width + n * 8 + g;
+    const bool live = n * 8 + g < p.width && member < p.members;
+    const int t = live ? member / p.groups : 0;
+    const int head = h * p.groups + (live ? member - t * p.groups : 0);
+    const __nv_bfloat16* row = p.q + ((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D;
+    uint2 w[D / 16];
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      w[k] = live ? *reinterpret_cast<const uint2*>(row + k * 16 + 4 * c) : make_uint2(0u, 0u);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(bf16_lo(w[k].x)), fabsf(bf16_hi(w[k].x)))),
+                  fmaxf(fabsf(bf16_lo(w[k].y)), fabsf(bf16_hi(w[k].y))));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^up in two factors: |up| reaches 147
+    const int exponent = static_cast<int>(__float_as_uint(top) >> 23);  // 0: zero or subnormal; 255: not finite
+    const int up = top > 0.f && exponent < 255 ? 14 + 127 - max(exponent, 1) : 0;
+    const int first = up / 2;
+    const float f0 = __uint_as_float(static_cast<uint32_t>(127 + first) << 23);
+    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up - first) << 23);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const uint32_t b0 = pack_f16x2(bf16_lo(w[k].x) * f0 * f1, bf16_hi(w[k].x) * f0 * f1);
+      const uint32_t b1 = pack_f16x2(bf16_lo(w[k].y) * f0 * f1, bf16_hi(w[k].y) * f0 * f1);
+      if constexpr (NG == 1) {
+        a.q[k][0] = b0;
+        a.q[k][1] = b1;
+      } else {
+        *reinterpret_cast<uint2*>(query + (n * 8 + g) * S::kQueryPitch + (k * 16 + 4 * c) * 2) = make_uint2(b0, b1);
+      }
+    }
+    const float mine = p.scale_log2 / f0 / f1;  // of column g; this thread's scores are 2c and 2c + 1
+    if constexpr (NG == 1) {
+      a.qs[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
+      a.qs[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+    } else if (c == 0) {
+      *reinterpret_cast<float*>(query + (n * 8 + g) * S::kQueryPitch + D * 2) = mine;
+    }
+  }
+  if constexpr (NG > 1) {
+    consumers_sync();
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        a.qs[n][e] = *reinterpret_cast<const float*>(query + (n * 8 + 2 * c + e) * S::kQueryPitch + D * 2);
+  }
+  clear<D, NG>(a);
 }
 
 // O^T += V^T P^T for this warp's 16 slots. Each register of a transposed load holds two dims of two
@@ -208,26 +285,40 @@ __device__ __forceinline__ bool any_nan(uint32_t tile, int warp, int lane) {
 // One 128-slot tile starting at slot `first`: this warp's 16 slots of it. `len`: slots of the row;
 // `position`: its first token's slot; ks, vs: the slice's scales.
 template <int D, int NG>
-__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, uint32_t kt, uint32_t vt, int first,
-                                            int len, int position, int chain, int chunk, float ks, float vs, int warp,
-                                            int lane) {
+__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const uint8_t* query, uint32_t kt,
+                                            uint32_t vt, int first, int len, int position, int chain, int chunk,
+                                            float ks, float vs, int warp, int lane) {
   const int slice = first + warp * 16;
   if (slice >= len) return;
   const int g = lane >> 2, c = lane & 3;
   const int row = warp * 16 + (lane & 15), half = lane >> 4;
-  float s[NG][4];
+  // two chains of products per column group: half the latency
+  float s[NG][4], s2[NG][4];
 #pragma unroll
-  for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+  for (int n = 0; n < NG; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     uint32_t r[4];
     ldmatrix_x4(kt + swizzled<D>(row, 2 * i + half), r[0], r[1], r[2], r[3]);
+    const uint32_t a0 = q8::e4m3x2_to_f16x2(r[0] & 0xffffu), a2 = q8::e4m3x2_to_f16x2(r[0] >> 16);
+    const uint32_t a1 = q8::e4m3x2_to_f16x2(r[1] & 0xffffu), a3 = q8::e4m3x2_to_f16x2(r[1] >> 16);
+    const uint32_t c0 = q8::e4m3x2_to_f16x2(r[2] & 0xffffu), c2 = q8::e4m3x2_to_f16x2(r[2] >> 16);
+    const uint32_t c1 = q8::e4m3x2_to_f16x2(r[3] & 0xffffu), c3 = q8::e4m3x2_to_f16x2(r[3] >> 16);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t a0 = q8::e4m3x2_to_f16x2(r[2 * j] & 0xffffu), a2 = q8::e4m3x2_to_f16x2(r[2 * j] >> 16);
-      const uint32_t a1 = q8::e4m3x2_to_f16x2(r[2 * j + 1] & 0xffffu), a3 = q8::e4m3x2_to_f16x2(r[2 * j + 1] >> 16);
-#pragma unroll
-      for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, a.q[n][2 * i + j][0], a.q[n][2 * i + j][1]);
+    for (int n = 0; n < NG; ++n) {
+      uint2 b0, b1;
+      if constexpr (NG == 1) {
+        b0 = make_uint2(a.q[2 * i][0], a.q[2 * i][1]);
+        b1 = make_uint2(a.q[2 * i + 1][0], a.q[2 * i + 1][1]);
+      } else {
+        const uint8_t* src = query + (n * 8 + g) * Smem<D, NG>::kQueryPitch + (i * 32 + 4 * c) * 2;
+        b0 = *reinterpret_cast<const uint2*>(src);
+        b1 = *reinterpret_cast<const uint2*>(src + 32);
+      }
+      mma_f16(s[n], a0, a1, a2, a3, b0.x, b0.y);
+      mma_f16(s2[n], c0, c1, c2, c3, b1.x, b1.y);
     }
   }
   const float lv = log2f(vs);  // -inf for a block of zeros
@@ -237,7 +328,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, ui
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] *= a.qs[n][e & 1] * ks;
+    for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * (a.qs[n][e & 1] * ks);
   }
   if (tail) {
 #pragma unroll
@@ -322,13 +413,11 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, ui
   value_product<D, NG>(a.o, vt, row, half, keep0, keep1, pb);
 }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32) : "memory"); }
-
-// Sums the eight warps' states (in warp order) and either writes the unit's output or leaves
-// its partials in `slot`.
-template <int D, int NG>
-__device__ void finish_run(State<D, NG>& a, const Params& p, int b, int h, int chunk, bool whole, size_t slot,
-                           float* red_o, float* red_stats, int warp, int lane) {
+// Sums the consumer warps' states in warp order, column group by column group: sink(in_chunk, d, O, M,
+// m, l) for every live column and dim.
+template <int D, int NG, typename Sink>
+__device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, float* red_stats, int members, int warp,
+                                             int lane, Sink sink) {
   const int g = lane >> 2, c = lane & 3, tid = threadIdx.x;
 #pragma unroll
   for (int n = 0; n < NG; ++n)
@@ -338,15 +427,14 @@ __device__ void finish_run(State<D, NG>& a, const Params& p, int b, int h, int c
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
       if (g == 0) {
-        float* st = red_stats + (warp * 32 + n * 8 + 2 * c + e) * 3;
+        float* st = red_stats + (warp * NG * 8 + n * 8 + 2 * c + e) * 3;
         st[0] = a.M[n][e], st[1] = a.m[n][e], st[2] = l;
       }
     }
-  const int members = min(p.width, p.members - chunk * p.width);
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     if (n * 8 >= members) break;  // uniform
-    consumers_sync();             // the last group's reads are done
+    if (n > 0) consumers_sync();  // the last group's reads are done
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       float* dst = red_o + (warp * D + 16 * k + 2 * g) * 8 + 2 * c;
@@ -354,70 +442,191 @@ __device__ void finish_run(State<D, NG>& a, const Params& p, int b, int h, int c
       *reinterpret_cast<float2*>(dst + 8) = make_float2(a.o[n][k][2], a.o[n][k][3]);
     }
     consumers_sync();
-    for (int e = tid; e < 8 * D; e += kWarps * 32) {
-      const int col = e / D, d = e % D, in_chunk = n * 8 + col;
+    // a thread's elements share a column (128 threads cover one or two columns at a time)
+#pragma unroll
+    for (int e0 = 0; e0 < 8 * D; e0 += kWarps * 32) {
+      const int e = e0 + tid, col = e / D, d = e % D, in_chunk = n * 8 + col;
       if (in_chunk >= members) break;
-      float M = -INFINITY, m = -INFINITY;
+      float wM[kWarps], wm[kWarps], M = -INFINITY, m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        M = fmaxf(M, red_stats[(w * 32 + in_chunk) * 3]);
-        m = fmaxf(m, red_stats[(w * 32 + in_chunk) * 3 + 1]);
+        const float* st = red_stats + (w * NG * 8 + in_chunk) * 3;
+        M = fmaxf(M, wM[w] = st[0]);
+        m = fmaxf(m, wm[w] = st[1]);
       }
       float O = 0.f, l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float* st = red_stats + (w * 32 + in_chunk) * 3;
-        O += red_o[(w * D + d) * 8 + col] * ex2(st[0] - pivot(M));
-        l += st[2] * ex2(st[1] - pivot(m));
+        O += red_o[(w * D + d) * 8 + col] * ex2(wM[w] - pivot(M));
+        l += red_stats[(w * NG * 8 + in_chunk) * 3 + 2] * ex2(wm[w] - pivot(m));
       }
-      if (whole) {
-        const int member = chunk * p.width + in_chunk;
-        const int t = member / p.groups, head = h * p.groups + member % p.groups;
-        p.out[((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D + d] =
-            __float2bfloat16_rn(finished(O, M, m, l));
-      } else {
-        p.acc[(slot * p.width + in_chunk) * D + d] = O;
-        if (d == 0) p.stats[slot * p.width + in_chunk] = make_float4(M, m, l, 0.f);
-      }
+      sink(in_chunk, d, O, M, m, l);
     }
   }
-  consumers_sync();  // red_stats is free for the next run
+}
+
+template <int D>
+__device__ __forceinline__ void write_out(const Params& p, int b, int h, int member, int d, float O, float M, float m,
+                                          float l) {
+  const int t = member / p.groups, head = h * p.groups + member - t * p.groups;
+  p.out[((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D + d] = __float2bfloat16_rn(finished(O, M, m, l));
 }
 
 template <int D, int NG>
-__global__ void __launch_bounds__(kThreads, 1)
-    attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                     const __grid_constant__ Params p) {
-  using S = Smem<D>;
-  constexpr int NS = S::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* stage_scales = reinterpret_cast<float*>(base + S::kRing);
-  float* red_o = reinterpret_cast<float*>(base + S::kRing + S::kScaleBytes);
-  float* red_stats = red_o + S::kRedO / 4;
-  int* cum = reinterpret_cast<int*>(red_stats + S::kRedStats / 4);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(cum) + S::kCum);
-  uint64_t* empty = full + NS;
-  volatile int* misc = reinterpret_cast<volatile int*>(empty + NS);  // [0..2]: first row, unit, tile; [3]: abort
+__device__ __forceinline__ void init_barriers(const Smem<D, NG>& sm, const CUtensorMap* kmap, const CUtensorMap* vmap) {
+  for (int s = 0; s < Smem<D, NG>::kStages; ++s) {
+    mbar_init(&sm.full[s], 1 + kScales);  // the tiles' bytes and the scale copies
+    mbar_init(&sm.empty[s], kWarps);
+  }
+  fence_barrier_init();
+  prefetch_tensormap(kmap);
+  prefetch_tensormap(vmap);
+  sm.misc[3] = 0;
+}
 
+// Producer warp: tile j of `pair` into stage k % stages. False after an abort.
+template <int D, int NG>
+__device__ __forceinline__ bool load_tile(const Smem<D, NG>& sm, const Params& p, const CUtensorMap* kmap,
+                                          const CUtensorMap* vmap, int k, int pair, int j, int lane) {
+  using S = Smem<D, NG>;
+  const int s = k % S::kStages;
+  bool ok = sm.misc[3] == 0;
+  if (ok && k >= S::kStages && !mbar_wait_bounded(&sm.empty[s], ((k / S::kStages) - 1) & 1)) {
+    raise_error(p.err, kErrTimeoutEmpty);
+    sm.misc[3] = 1;
+    ok = false;
+  }
+  if (!__all_sync(0xffffffffu, ok)) return false;
+  if (lane == 0) {
+    uint8_t* kt = sm.ring + s * 2 * S::kTileBytes;
+    const int row = pair * p.capacity + j * kTile;
+    mbar_arrive_expect_tx(&sm.full[s], 2 * S::kTileBytes);
+    tma_load_2d(kt, kmap, &sm.full[s], 0, row);
+    tma_load_2d(kt + S::kTileBytes, vmap, &sm.full[s], 0, row);
+  }
+  if (lane < kScales) {
+    const int i = min((j * kTile + (lane % kWarps) * 16) / p.block, p.blocks - 1);
+    const float* src = (lane < kWarps ? p.key_scales : p.value_scales) + static_cast<size_t>(pair) * p.blocks + i;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sm.scales + s * kScales + lane)), "l"(src)
+                 : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[s])) : "memory");
+  }
+  return true;
+}
+
+// After an abort: copies in flight land before the CTA's shared memory is released.
+template <int D, int NG>
+__device__ __forceinline__ void drain(const Smem<D, NG>& sm, int issued) {
+  constexpr int NS = Smem<D, NG>::kStages;
+  if (sm.misc[3] != 0)
+    for (int k = issued > NS ? issued - NS : 0; k < issued; ++k) mbar_wait_bounded(&sm.full[k % NS], (k / NS) & 1);
+}
+
+// Consumer warp: tile j of a row with `len` slots from stage k % stages. After an abort the barriers
+// that follow are still taken, on whatever the stage holds.
+template <int D, int NG>
+__device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>& sm, const Params& p, int k, int j,
+                                             int len, int position, int chain, int chunk, int warp, int lane) {
+  using S = Smem<D, NG>;
+  const int s = k % S::kStages;
+  if (sm.misc[3] == 0 && !mbar_wait_bounded(&sm.full[s], (k / S::kStages) & 1)) {
+    raise_error(p.err, kErrTimeoutFull);
+    sm.misc[3] = 1;
+  }
+  __syncwarp();
+  const uint32_t kt = smem_u32(sm.ring + s * 2 * S::kTileBytes);
+  const float ks = sm.scales[s * kScales + warp], vs = sm.scales[s * kScales + kWarps + warp];
+  attend_tile<D, NG>(a, p, sm.query, kt, kt + S::kTileBytes, j * kTile, len, position, chain, chunk, ks, vs, warp, lane);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&sm.empty[s]);
+}
+
+__device__ __forceinline__ int first_position(const Params& p, int b) {
+  return static_cast<int>(min(p.position[p.per_row ? b : 0], static_cast<int64_t>(p.capacity)));
+}
+
+// ------------------------------------------------------------------------------ cluster form
+template <int D, int NG>
+__global__ void __launch_bounds__(kThreads, 2)
+    cluster_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                   const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const Smem<D, NG> sm(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = gridDim.x, rank = blockIdx.x;  // cluster dims (C, 1, 1)
+  const int pair = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks;
+  const int b = pair / p.kv_heads, h = pair % p.kv_heads;
+  cluster_arrive_relaxed();  // this CTA runs: its shared memory may be written once all have said so
+  if (warp == kWarps && lane == 0) init_barriers(sm, &kmap, &vmap);
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const int len = row_length(p, b), n = tiles_of(len);
+  const int count = n > rank ? (n - rank + C - 1) / C : 0;  // tiles rank, rank + C, ...
+  if (warp == kWarps) {
+    int k = 0;
+    while (k < count && load_tile(sm, p, &kmap, &vmap, k, pair, rank + k * C, lane)) ++k;
+    drain(sm, k);
+    __syncwarp();
+    cluster_wait();  // every thread of the cluster takes the same two barrier phases
+    cluster_sync();
+    return;
+  }
+  const int position = first_position(p, b);
+  const int chain = p.chain != nullptr ? static_cast<int>(p.chain[b]) : 1;
+  const int members = min(p.width, p.members - chunk * p.width);
+  State<D, NG> a;
+  start_unit<D, NG>(a, p, sm.query, b, h, chunk, warp, lane);
+  for (int k = 0; k < count; ++k)
+    consume_tile(a, sm, p, k, rank + k * C, len, position, chain, chunk, warp, lane);
+  const int total = members * D, share = (total + C - 1) / C;
+  cluster_wait();  // every CTA of the cluster runs
+  reduce_warps<D, NG>(a, sm.red_o, sm.red_stats, members, warp, lane,
+                      [&](int col, int d, float O, float M, float m, float l) {
+                        const int e = col * D + d, owner = e / share;
+                        st_cluster_f32(map_shared(smem_u32(sm.recv_o + rank * share + e - owner * share), owner), O);
+                        if (d < C) {  // one thread per rank passes this column's statistics on
+                          const uint32_t at = map_shared(smem_u32(sm.recv_stats + (rank * NG * 8 + col) * 3), d);
+                          st_cluster_f32(at, M);
+                          st_cluster_f32(at + 4, m);
+                          st_cluster_f32(at + 8, l);
+                        }
+                      });
+  cluster_sync();  // every partial has landed; nobody touches another CTA's memory after this
+  const int low = rank * share, high = min(total, low + share);
+  for (int e = low + static_cast<int>(threadIdx.x); e < high; e += kWarps * 32) {
+    const int col = e / D;
+    float M = -INFINITY, m = -INFINITY, O = 0.f, l = 0.f;
+    for (int q = 0; q < C; ++q) {
+      M = fmaxf(M, sm.recv_stats[(q * NG * 8 + col) * 3]);
+      m = fmaxf(m, sm.recv_stats[(q * NG * 8 + col) * 3 + 1]);
+    }
+    for (int q = 0; q < C; ++q) {
+      const float* st = sm.recv_stats + (q * NG * 8 + col) * 3;
+      O += sm.recv_o[q * share + e - low] * ex2(st[0] - pivot(M));
+      l += st[2] * ex2(st[1] - pivot(m));
+    }
+    write_out<D>(p, b, h, chunk * p.width + col, e % D, O, M, m, l);
+  }
+}
+
+// --------------------------------------------------------------------------- persistent form
+template <int D, int NG>
+__global__ void __launch_bounds__(kThreads, 2)
+    persistent_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const Smem<D, NG> sm(smem_raw);
+  const int* cum = sm.cum;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int B = p.batch, per_row = p.kv_heads * p.chunks;  // units of a row
-  if (warp == kWarps && lane == 0) {
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1 + kScales);  // the tiles' bytes and 16 scale copies
-      mbar_init(&empty[s], kWarps);
-    }
-    fence_barrier_init();
-    prefetch_tensormap(&kmap);
-    prefetch_tensormap(&vmap);
-    misc[3] = 0;
-  }
+  if (warp == kWarps && lane == 0) init_barriers(sm, &kmap, &vmap);
   pdl_wait();
   pdl_trigger();
   // ---- plan: tiles before each row, this CTA's slice and where it begins ----
   if (warp == 0) {
     int running = 0;
-    if (lane == 0) cum[0] = 0;
+    if (lane == 0) sm.cum[0] = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
       const int b = b0 + lane;
       int x = b < B ? tiles_of(row_length(p, b)) : 0;
@@ -426,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      if (b < B) cum[b + 1] = running + x;
+      if (b < B) sm.cum[b + 1] = running + x;
       running += __shfl_sync(0xffffffffu, x, 31);
     }
   }
@@ -442,47 +651,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                        t0 < static_cast<long long>(per_row) * cum[b + 1];
       if (hit) {
         const int n = cum[b + 1] - cum[b];
-        const long long off = t0 - static_cast<long long>(per_row) * cum[b];
-        misc[0] = b;
-        misc[1] = static_cast<int>(off / n);
-        misc[2] = static_cast<int>(off % n);
+        const int off = static_cast<int>(t0 - static_cast<long long>(per_row) * cum[b]);  // < 2^31: tiles of one row
+        sm.misc[0] = b;
+        sm.misc[1] = off / n;
+        sm.misc[2] = off % n;
       }
       if (__any_sync(0xffffffffu, hit)) break;
     }
   }
   __syncthreads();
-  int b = misc[0], u = misc[1], j = misc[2];  // row, unit of the row (KV head, chunk), tile
+  int b = sm.misc[0], u = sm.misc[1], j = sm.misc[2];  // row, unit of the row (KV head, chunk), tile
   int n = cum[b + 1] - cum[b];
 
   if (warp == kWarps) {
-    // ================================ producer ================================
-    int issued = 0;
-    for (int k = 0; k < count; ++k) {
-      const int s = k % NS;
-      bool ok = misc[3] == 0;
-      if (ok && k >= NS && !mbar_wait_bounded(&empty[s], ((k / NS) - 1) & 1)) {
-        if (lane == 0) raise_error(p.err, kErrTimeoutEmpty);
-        misc[3] = 1;
-        ok = false;
-      }
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const size_t pair = static_cast<size_t>(b) * p.kv_heads + u / p.chunks;
-      if (lane == 0) {
-        uint8_t* kt = base + s * 2 * S::kTileBytes;
-        const int row = static_cast<int>(pair * p.capacity) + j * kTile;
-        mbar_arrive_expect_tx(&full[s], 2 * S::kTileBytes);
-        tma_load_2d(kt, &kmap, &full[s], 0, row);
-        tma_load_2d(kt + S::kTileBytes, &vmap, &full[s], 0, row);
-      }
-      if (lane < kScales) {
-        const int i = min((j * kTile + (lane & 7) * 16) / p.block, p.blocks - 1);
-        const float* src = (lane < 8 ? p.key_scales : p.value_scales) + pair * p.blocks + i;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stage_scales + s * kScales + lane)),
-                     "l"(src)
-                     : "memory");
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
-      }
-      issued = k + 1;
+    int k = 0;
+    for (; k < count; ++k) {
+      if (!load_tile(sm, p, &kmap, &vmap, k, b * p.kv_heads + u / p.chunks, j, lane)) break;
       if (++j == n) {
         j = 0;
         if (++u == per_row) {
@@ -493,70 +677,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    // after an abort: let the copies in flight land before the block's shared memory is released
-    if (misc[3] != 0)
-      for (int k = issued > NS ? issued - NS : 0; k < issued; ++k) mbar_wait_bounded(&full[k % NS], (k / NS) & 1);
+    drain(sm, k);
     return;
   }
 
-  // ================================ consumers ================================
-  int len = row_length(p, b);
-  int position = static_cast<int>(min(p.position[p.per_row ? b : 0], static_cast<int64_t>(p.capacity)));
-  int chain = p.chain != nullptr ? static_cast<int>(p.chain[b]) : 1;
-  int run_first = j;
+  int run_first = 0, len = 0, position = 0, chain = 1;
+  bool starts = true;
   State<D, NG> a;
-  start_unit<D, NG>(a, p, b, u / p.chunks, u % p.chunks, lane);
   for (int k = 0; k < count; ++k) {
-    const int s = k % NS;
-    bool ok = misc[3] == 0;
-    if (ok && !mbar_wait_bounded(&full[s], (k / NS) & 1)) {
-      raise_error(p.err, kErrTimeoutFull);
-      misc[3] = 1;
+    if (starts) {
+      n = cum[b + 1] - cum[b];
+      len = row_length(p, b);
+      position = first_position(p, b);
+      if (p.chain != nullptr) chain = static_cast<int>(p.chain[b]);
+      run_first = j;
+      start_unit<D, NG>(a, p, sm.query, b, u / p.chunks, u % p.chunks, warp, lane);
     }
-    const uint32_t kt = smem_u32(base + s * 2 * S::kTileBytes);
-    // an aborted launch still takes every barrier below, on whatever the stage holds
-    const float ks = stage_scales[s * kScales + warp], vs = stage_scales[s * kScales + 8 + warp];
-    attend_tile<D, NG>(a, p, kt, kt + S::kTileBytes, j * kTile, len, position, chain, u % p.chunks, ks, vs, warp, lane);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-    const int run_b = b, run_u = u, run_last = j, run_n = n;
-    bool ends = k == count - 1;
+    consume_tile(a, sm, p, k, j, len, position, chain, u % p.chunks, warp, lane);
+    const int run_b = b, run_u = u, run_last = j;
+    starts = k == count - 1;
     if (++j == n) {
       j = 0;
-      ends = true;
+      starts = true;
       if (++u == per_row) {
         u = 0;
         do ++b;
         while (b < B && cum[b + 1] == cum[b]);
       }
     }
-    if (!ends) continue;
+    if (!starts) continue;
+    // the run ends: its unit's output, or partials for the merge
+    const int h = run_u / p.chunks, chunk = run_u % p.chunks;
     const size_t slot = blockIdx.x + static_cast<size_t>(run_b) * per_row + run_u;
-    finish_run<D, NG>(a, p, run_b, run_u / p.chunks, run_u % p.chunks, run_first == 0 && run_last == run_n - 1, slot,
-                      red_o, red_stats, warp, lane);
-    if (k != count - 1) {
-      n = cum[b + 1] - cum[b];
-      len = row_length(p, b);
-      position = static_cast<int>(min(p.position[p.per_row ? b : 0], static_cast<int64_t>(p.capacity)));
-      chain = p.chain != nullptr ? static_cast<int>(p.chain[b]) : 1;
-      run_first = j;
-      start_unit<D, NG>(a, p, b, u / p.chunks, u % p.chunks, lane);
-    }
+    const bool whole = run_first == 0 && run_last == n - 1;
+    consumers_sync();  // the last run's reductions are read
+    reduce_warps<D, NG>(a, sm.red_o, sm.red_stats, min(p.width, p.members - chunk * p.width), warp, lane,
+                        [&](int col, int d, float O, float M, float m, float l) {
+                          if (whole) {
+                            write_out<D>(p, run_b, h, chunk * p.width + col, d, O, M, m, l);
+                          } else {
+                            p.acc[(slot * p.width + col) * D + d] = O;
+                            if (d == 0) p.stats[slot * p.width + col] = make_float4(M, m, l, 0.f);
+                          }
+                        });
   }
 }
 
-// One CTA per unit: merges the runs of the CTAs that shared it, in CTA order, and writes the
-// zeros of empty rows.
-constexpr int kMergeThreads = 128;
+// One CTA per (unit, 8 columns): merges the runs of the CTAs that shared the unit, in CTA order, and
+// writes the zeros of empty rows. The plan is worked out before the wait (the positions were
+// there before the first launch passed its own); after it a unit of at most four runs takes one
+// round trip to L2: statistics and accumulators are loaded together.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeRuns = 4;
 
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ Params p) {
   __shared__ int s_before, s_total;
-  pdl_wait();
-  pdl_trigger();
   const int per_row = p.kv_heads * p.chunks;
   const int b = blockIdx.x / per_row, u = blockIdx.x % per_row;
-  const int h = u / p.chunks, chunk = u % p.chunks;
+  const int h = u / p.chunks, chunk = u % p.chunks, col0 = blockIdx.y * 8;
   if (threadIdx.x == 0) s_before = s_total = 0;
   __syncthreads();
   int before = 0, total = 0;
@@ -569,32 +748,49 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   if (total) atomicAdd(&s_total, total);
   __syncthreads();
   const int n = tiles_of(row_length(p, b));
-  const int members = min(p.width, p.members - chunk * p.width);
+  const int members = min(8, min(p.width, p.members - chunk * p.width) - col0);
   const long long T = static_cast<long long>(per_row) * s_total;
   const long long first = static_cast<long long>(per_row) * s_before + static_cast<long long>(u) * n;
   const int lo = n > 0 ? slice_owner(T, first, p.ctas) : 0, hi = n > 0 ? slice_owner(T, first + n - 1, p.ctas) : 0;
+  const bool sparse = T < p.ctas;  // some slices are empty: their CTAs wrote nothing
+  pdl_wait();
+  pdl_trigger();
   if (n > 0 && lo == hi) return;  // one run covered the unit and wrote its output
   for (int e = threadIdx.x; e < members * D; e += kMergeThreads) {
-    const int in_chunk = e / D, d = e % D, member = chunk * p.width + in_chunk;
+    const int col = col0 + e / D, d = e % D;
     float M = -INFINITY, m = -INFINITY, O = 0.f, l = 0.f;
     if (n > 0) {
-      for (int i = lo; i <= hi; ++i) {
-        if (slice_start(T, i, p.ctas) >= slice_start(T, i + 1, p.ctas)) continue;  // an empty slice wrote nothing
-        const float4 st = p.stats[(static_cast<size_t>(i) + blockIdx.x) * p.width + in_chunk];
-        M = fmaxf(M, st.x);
-        m = fmaxf(m, st.y);
-      }
-      for (int i = lo; i <= hi; ++i) {
-        if (slice_start(T, i, p.ctas) >= slice_start(T, i + 1, p.ctas)) continue;
-        const size_t at = (static_cast<size_t>(i) + blockIdx.x) * p.width + in_chunk;
-        const float4 st = p.stats[at];
-        O += p.acc[at * D + d] * ex2(st.x - pivot(M));
-        l += st.z * ex2(st.y - pivot(m));
+      const float4* st = p.stats + (static_cast<size_t>(lo) + blockIdx.x) * p.width + col;
+      const float* acc = p.acc + ((static_cast<size_t>(lo) + blockIdx.x) * p.width + col) * D + d;
+      for (int i0 = 0; i0 <= hi - lo; i0 += kMergeRuns) {
+        float4 s[kMergeRuns];
+        float v[kMergeRuns];
+        float tM = M, tm = m;
+#pragma unroll
+        for (int i = 0; i < kMergeRuns; ++i) {
+          const int run = i0 + i;
+          const bool on = run <= hi - lo &&
+                          !(sparse && slice_start(T, lo + run, p.ctas) == slice_start(T, lo + run + 1, p.ctas));
+          s[i] = on ? __ldcg(st + static_cast<size_t>(run) * p.width) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+          v[i] = on ? __ldcg(acc + static_cast<size_t>(run) * p.width * D) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kMergeRuns; ++i) {
+          tM = fmaxf(tM, s[i].x);
+          tm = fmaxf(tm, s[i].y);
+        }
+        O *= ex2(M - pivot(tM));
+        l *= ex2(m - pivot(tm));
+        M = tM;
+        m = tm;
+#pragma unroll
+        for (int i = 0; i < kMergeRuns; ++i) {
+          O += v[i] * ex2(s[i].x - pivot(M));
+          l += s[i].z * ex2(s[i].y - pivot(m));
+        }
       }
     }
-    const int t = member / p.groups, head = h * p.groups + member % p.groups;
-    p.out[((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D + d] =
-        __float2bfloat16_rn(finished(O, M, m, l));
+    write_out<D>(p, b, h, chunk * p.width + col, d, O, M, m, l);
   }
 }
 
@@ -632,25 +828,80 @@ int shape(Params* p, int batch, int tokens, int q_heads, int kv_heads, int head_
   p->capacity = capacity;
   p->block = block;
   p->blocks = (capacity + block - 1) / block;
-  p->ctas = sm_count();
+  p->ctas = 2 * sm_count();
   chunk_members(p, head_dim);
-  return static_cast<long long>(batch) * kv_heads * p->chunks >= (1ll << 31) ? FB_ERR_SHAPE : FB_OK;
+  const long long row_units = static_cast<long long>(kv_heads) * p->chunks;
+  return batch * row_units >= (1ll << 31) || row_units * tiles_of(capacity) >= (1ll << 31) ? FB_ERR_SHAPE : FB_OK;
+}
+
+constexpr int kMaxDevices = 64;
+
+template <int D, int NG>
+bool configure() {
+  static bool configured[kMaxDevices] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < kMaxDevices && configured[dev]) return true;
+  const int bytes = Smem<D, NG>::kTotal;
+  if (cudaFuncSetAttribute(cluster_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(persistent_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return false;
+  if (cudaFuncSetAttribute(cluster_kernel<D, NG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    cudaGetLastError();  // no clusters above 8: the occupancy query then reports none
+  if (dev < kMaxDevices) configured[dev] = true;
+  return true;
+}
+
+// Clusters of c CTAs that the device holds at once (0 if unknown), kept per device.
+template <int D, int NG>
+int resident_clusters(int c) {
+  static int cache[kMaxDevices][kMaxCluster + 1] = {};  // count + 1; 0: not asked
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < kMaxDevices && cache[dev][c] != 0) return cache[dev][c] - 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(c, 1);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<D, NG>::kTotal;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, cluster_kernel<D, NG>, &cfg) != cudaSuccess || n < 0) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (dev < kMaxDevices) cache[dev][c] = n + 1;
+  return n;
+}
+
+// The cluster size of a launch, 0 for the persistent form: the largest whose clusters are all
+// resident at once, no larger than the cache has tiles.
+template <int D, int NG>
+int cluster_size(const Params& p) {
+  const int units = p.batch * p.kv_heads * p.chunks;
+  if (units > sm_count() || units > 65535) return 0;
+  const int tiles = tiles_of(p.capacity);
+  for (int c = tiles < kMaxCluster ? tiles : kMaxCluster; c >= 1; --c)
+    if (resident_clusters<D, NG>(c) >= units) return c;
+  return 0;
 }
 
 template <int D, int NG>
 int launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, cudaStream_t stream) {
-  static bool configured[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return FB_ERR_LAUNCH;
-  if (dev >= 64 || !configured[dev]) {
-    if (cudaFuncSetAttribute(attention_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kTotal) !=
-        cudaSuccess)
-      return FB_ERR_LAUNCH;
-    if (dev < 64) configured[dev] = true;
-  }
-  const int st = launch_ex(attention_kernel<D, NG>, dim3(p.ctas), dim3(kThreads), Smem<D>::kTotal, stream, 1, km, vm, p);
+  if (!configure<D, NG>()) return FB_ERR_LAUNCH;
+  const int units = p.batch * p.kv_heads * p.chunks;
+  constexpr int bytes = Smem<D, NG>::kTotal;
+  const int c = cluster_size<D, NG>(p);
+  if (c > 0)
+    return launch_ex(cluster_kernel<D, NG>, dim3(c, units), dim3(kThreads), bytes, stream, c, km, vm, p);
+  const int st = launch_ex(persistent_kernel<D, NG>, dim3(p.ctas), dim3(kThreads), bytes, stream, 1, km, vm, p);
   if (st != FB_OK) return st;
-  return launch_ex(merge_kernel<D>, dim3(p.batch * p.kv_heads * p.chunks), dim3(kMergeThreads), 0, stream, 1, p);
+  return launch_ex(merge_kernel<D>, dim3(units, (p.width + 7) / 8), dim3(kMergeThreads), 0, stream, 1, p);
 }
 
 template <int D>
