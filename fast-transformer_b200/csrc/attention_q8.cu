@@ -14,11 +14,12 @@
 // fp32. Q is scaled by a power of two to f16's range (exact for any bf16 row).
 //
 // Bound by the bytes of codes. Members = the T * G query heads that share a KV head, in groups of
-// 8 NG columns; a unit = (row, KV head, member group); its tiles are 64 slots of K and V. A CTA is
-// a producer warp (one lane issues a TMA load per K and V tile, 8 lanes copy the tile's scales
-// with cp.async; both complete on the stage's mbarrier) and four consumer warps of 16 slots each:
-// S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a score passes it by more than 8, one
-// vote), O^T += V^T P^T. Two CTAs share an SM, so that one streams while the other starts or ends.
+// 8 NG columns; a unit = (row, KV head, member group); its tiles are 128 slots of K and V. A CTA is
+// a producer warp (one lane issues a TMA load per K and V tile, 16 lanes copy the tile's scales
+// with cp.async; both complete on the stage's mbarrier) and four consumer warps of two 16-slot
+// slices each: S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a score passes it by more
+// than 8, one vote), O^T += V^T P^T. Two CTAs share an SM: one streams while the other starts or
+// ends.
 //  * Few units: a cluster of C CTAs per unit (interleaved tiles), merged by pushing each
 //    partial to its output's owner through distributed shared memory: one launch, no workspace.
 //  * Many units: a persistent grid cuts the tiles of all units into equal contiguous slices, so
@@ -30,11 +31,12 @@
 namespace fb {
 namespace attn8 {
 
-constexpr int kWarps = 4;  // consumers: 16 slots of a tile each
-constexpr int kTile = 16 * kWarps;
+constexpr int kWarps = 4;  // consumers
+constexpr int kSlices = 2 * kWarps;  // of 16 slots: warp w takes slices 2 w and 2 w + 1
+constexpr int kTile = 16 * kSlices;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kMaxBatch = 1024;
-constexpr int kScales = 2 * kWarps;  // per stage: K and V scale of each 16-slot slice
+constexpr int kScales = 2 * kSlices;  // per stage: K and V scale of each 16-slot slice
 constexpr int kMaxCluster = 16;      // above 8: the non-portable cluster size attribute
 constexpr float kSlack = 8.f;        // log2 a score may pass the pivot by: p <= 2^8, exact enough in f16
 
@@ -107,12 +109,13 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) {
 template <int D, int NG>
 struct Smem {
   static constexpr int kTileBytes = kTile * D;
-  static constexpr int kStages = D == 128 ? 5 : 8;
+  // two CTAs per SM (asserted below): what the buffers of more column groups leave
+  static constexpr int kStages = D == 128 ? (NG == 1 ? 3 : 2) : 5;
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kScaleBytes = kStages * kScales * 4;
   static constexpr int kQueryPitch = D * 2 + 32;  // f16 query rows, padded against bank conflicts
-  static constexpr int kQuery = NG * 8 * kQueryPitch;
-  static constexpr int kRedO = kWarps * D * 8 * 4;           // one 8-column group of every warp
+  static constexpr int kQuery = NG == 1 ? 0 : NG * 8 * kQueryPitch;
+  static constexpr int kRedO = kWarps * D / 2 * 8 * 4;       // half the dims of an 8-column group of every warp
   static constexpr int kRedStats = kWarps * NG * 8 * 3 * 4;  // M, m, l
   // persistent form: tile counts before each row; cluster form: O received as an owner
   // ([rank][chunk], C * ceil(n / C) <= n + C - 1 values) and every rank's M, m, l
@@ -122,6 +125,7 @@ struct Smem {
   static constexpr int kShared = kCum > kRecvO + kRecvStats ? kCum : kRecvO + kRecvStats;
   static constexpr int kBars = 2 * kStages * 8;
   static constexpr int kTotal = 1024 + kRing + kScaleBytes + kQuery + kRedO + kRedStats + kShared + kBars + 32;
+  static_assert(kTotal + 1024 <= 228 * 1024 / 2, "two CTAs per SM");
   static_assert((kScaleBytes + kQuery + kRedO + kRedStats + kShared) % 16 == 0, "mbarrier alignment");
 
   uint8_t* ring;
@@ -241,25 +245,34 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
   clear<D, NG>(a);
 }
 
-// O^T += V^T P^T for this warp's 16 slots. Each register of a transposed load holds two dims of two
-// slots; one byte permute and two conversions make the A fragments of dims 2g (rows 0-7 of the
-// product) and 2g + 1 (rows 8-15). keep0 / keep1 mask the bytes of slots (2c, 2c+1) and 8 later.
+// O^T += V^T P^T for 16 slots (`row`: this lane's row of the tile, `half`: its 16-byte chunk's parity).
+// Each register of a transposed load holds two dims of two slots; one byte permute and two
+// conversions make the A fragments of dims 2g (rows 0-7 of the product) and 2g + 1 (rows 8-15).
+// pick0 / pick1 are the permutes of slots (2c, 2c + 1) and 8 later: kPick, or with selectors of 4
+// (a zero byte) for slots left out.
+constexpr uint32_t kPick = 0x3120u;
+
 template <int D, int NG>
 __device__ __forceinline__ void value_product(float (&o)[NG][D / 16][4], uint32_t tile, int row, int half,
-                                              uint32_t keep0, uint32_t keep1, const uint32_t (&pb)[NG][2]) {
+                                              uint32_t pick0, uint32_t pick1, const uint32_t (&pb)[NG][2]) {
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     uint32_t r[4];
     ldmatrix_x4_trans(tile + swizzled<D>(row, 2 * i + half), r[0], r[1], r[2], r[3]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint32_t w0 = __byte_perm(r[2 * j] & keep0, 0, 0x3120), w1 = __byte_perm(r[2 * j + 1] & keep1, 0, 0x3120);
-      const uint32_t a0 = q8::e4m3x2_to_f16x2(w0 & 0xffffu), a1 = q8::e4m3x2_to_f16x2(w0 >> 16);
-      const uint32_t a2 = q8::e4m3x2_to_f16x2(w1 & 0xffffu), a3 = q8::e4m3x2_to_f16x2(w1 >> 16);
+      uint32_t a0, a1, a2, a3;
+      q8::e4m3x4_to_f16x4(__byte_perm(r[2 * j], 0, pick0), a0, a1);
+      q8::e4m3x4_to_f16x4(__byte_perm(r[2 * j + 1], 0, pick1), a2, a3);
 #pragma unroll
       for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * i + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
     }
   }
+}
+
+// The permute that keeps slot 2c (result bytes 0 and 2) and slot 2c + 1 (bytes 1 and 3), or not.
+__device__ __forceinline__ uint32_t pick_slots(bool even, bool odd) {
+  return (even ? kPick & 0x0f0fu : 0x0404u) | (odd ? kPick & 0xf0f0u : 0x4040u);
 }
 
 // Whether token t of a row sees `slot`: the prefix [0, position] and, past it, the chain's tokens up
@@ -269,148 +282,185 @@ __device__ __forceinline__ bool sees(int slot, int len, int position, int t, int
   return slot <= position || (t < chain ? slot <= position + t : slot == position + t);
 }
 
-// Whether this warp's 16 rows of a tile hold a NaN code.
+// Whether rows [row0, row0 + 16) of a tile hold a NaN code.
 template <int D>
-__device__ __forceinline__ bool any_nan(uint32_t tile, int warp, int lane) {
+__device__ __forceinline__ bool any_nan(uint32_t tile, int row0, int lane) {
   bool found = false;
   for (int i = lane; i < 16 * D / 4; i += 32) {
     uint32_t w;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(tile + warp * 16 * D + i * 4) : "memory");
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(tile + row0 * D + i * 4) : "memory");
     w &= 0x7f7f7f7fu;  // a byte of 0x7f: adding 1 reaches its top bit
     found = found || ((w + 0x01010101u) & 0x80808080u) != 0;
   }
   return __any_sync(0xffffffffu, found);
 }
 
-// One 128-slot tile starting at slot `first`: this warp's 16 slots of it. `len`: slots of the row;
-// `position`: its first token's slot; ks, vs: the slice's scales.
+// log2 of a scale; exact for powers of two, -inf for 0.
+__device__ __forceinline__ float log2_scale(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// This warp's two slices of the 128-slot tile that starts at slot `first`. `len`: slots of the row;
+// `position`: its first token's slot; scales: the tile's, K then V. Up to two column groups the
+// slices run side by side (two independent chains hide each other's latency), else in turn.
 template <int D, int NG>
-__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const uint8_t* query, uint32_t kt,
-                                            uint32_t vt, int first, int len, int position, int chain, int chunk,
-                                            float ks, float vs, int warp, int lane) {
-  const int slice = first + warp * 16;
-  if (slice >= len) return;
-  const int g = lane >> 2, c = lane & 3;
-  const int row = warp * 16 + (lane & 15), half = lane >> 4;
-  // two chains of products per column group: half the latency
-  float s[NG][4], s2[NG][4];
+__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const uint8_t* query,
+                                            const float* scales, uint32_t kt, uint32_t vt, int first, int len,
+                                            int position, int chain, int chunk, int warp, int lane) {
+  constexpr int H = NG <= 2 ? 2 : 1;
+  const int g = lane >> 2, c = lane & 3, half = lane >> 4;
+#pragma unroll 1
+  for (int s0 = 0; s0 < 2; s0 += H) {
+    const int slice = first + (warp * 2 + s0) * 16;
+    if (slice >= len) return;
+    const int row = (warp * 2 + s0) * 16 + (lane & 15);
+    float s[H][NG][4], s2[H][NG][4];
 #pragma unroll
-  for (int n = 0; n < NG; ++n)
+    for (int x = 0; x < H; ++x)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    uint32_t r[4];
-    ldmatrix_x4(kt + swizzled<D>(row, 2 * i + half), r[0], r[1], r[2], r[3]);
-    const uint32_t a0 = q8::e4m3x2_to_f16x2(r[0] & 0xffffu), a2 = q8::e4m3x2_to_f16x2(r[0] >> 16);
-    const uint32_t a1 = q8::e4m3x2_to_f16x2(r[1] & 0xffffu), a3 = q8::e4m3x2_to_f16x2(r[1] >> 16);
-    const uint32_t c0 = q8::e4m3x2_to_f16x2(r[2] & 0xffffu), c2 = q8::e4m3x2_to_f16x2(r[2] >> 16);
-    const uint32_t c1 = q8::e4m3x2_to_f16x2(r[3] & 0xffffu), c3 = q8::e4m3x2_to_f16x2(r[3] >> 16);
+        for (int e = 0; e < 4; ++e) s[x][n][e] = s2[x][n][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      uint2 b0[NG], b1[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        if constexpr (NG == 1) {
+          b0[n] = make_uint2(a.q[2 * i][0], a.q[2 * i][1]);
+          b1[n] = make_uint2(a.q[2 * i + 1][0], a.q[2 * i + 1][1]);
+        } else {
+          const uint8_t* src = query + (n * 8 + g) * Smem<D, NG>::kQueryPitch + (i * 32 + 4 * c) * 2;
+          b0[n] = *reinterpret_cast<const uint2*>(src);
+          b1[n] = *reinterpret_cast<const uint2*>(src + 32);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < H; ++x) {
+        uint32_t r[4], k0[4], k1[4];
+        ldmatrix_x4(kt + swizzled<D>(row + 16 * x, 2 * i + half), r[0], r[1], r[2], r[3]);
+        q8::e4m3x4_to_f16x4(r[0], k0[0], k0[2]);
+        q8::e4m3x4_to_f16x4(r[1], k0[1], k0[3]);
+        q8::e4m3x4_to_f16x4(r[2], k1[0], k1[2]);
+        q8::e4m3x4_to_f16x4(r[3], k1[1], k1[3]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {  // two chains of products per group: half the latency
+          mma_f16(s[x][n], k0[0], k0[1], k0[2], k0[3], b0[n].x, b0[n].y);
+          mma_f16(s2[x][n], k1[0], k1[1], k1[2], k1[3], b1[n].x, b1[n].y);
+        }
+      }
+    }
+    float lv[H];
+#pragma unroll
+    for (int x = 0; x < H; ++x) {
+      const bool live = slice + 16 * x < len;  // past the row a scale can be anything
+      const float ks = live ? scales[warp * 2 + s0 + x] : 1.f;
+      lv[x] = live ? log2_scale(scales[kSlices + warp * 2 + s0 + x]) : 0.f;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][n][e] = (s[x][n][e] + s2[x][n][e]) * (a.qs[n][e & 1] * ks);
+    }
+    // every member sees slots [0, position]; past them the chain rule decides per token
+    const bool tail = slice + 16 * H > (p.chain != nullptr ? position + 1 : len);
+    if (tail) {
+#pragma unroll
+      for (int x = 0; x < H; ++x)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int slot = slice + 16 * x + g + (e >> 1) * 8;
+            const int t = p.chain != nullptr ? (chunk * p.width + n * 8 + 2 * c + (e & 1)) / p.groups : 0;
+            if (!sees(slot, len, position, t, chain)) s[x][n][e] = -INFINITY;
+          }
+    }
+    bool moves = false;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < H; ++x)
+          moves = moves || fmaxf(s[x][n][e], s[x][n][e + 2]) > fminf(a.m[n][e], a.M[n][e] - lv[x]) + kSlack;
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = a.m[n][e], M = a.M[n][e];
+#pragma unroll
+          for (int x = 0; x < H; ++x) {
+            float top = fmaxf(s[x][n][e], s[x][n][e + 2]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            m = fmaxf(m, top);
+            M = fmaxf(M, top + lv[x]);
+          }
+          const float fl = ex2(a.m[n][e] - pivot(m)), fo = ex2(a.M[n][e] - pivot(M));
+          a.m[n][e] = m;
+          a.M[n][e] = M;
+          a.l[n][e] *= fl;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            a.o[n][k][e] *= fo;
+            a.o[n][k][e + 2] *= fo;
+          }
+        }
+    }
+    uint32_t pb[H][NG][2];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      uint2 b0, b1;
-      if constexpr (NG == 1) {
-        b0 = make_uint2(a.q[2 * i][0], a.q[2 * i][1]);
-        b1 = make_uint2(a.q[2 * i + 1][0], a.q[2 * i + 1][1]);
-      } else {
-        const uint8_t* src = query + (n * 8 + g) * Smem<D, NG>::kQueryPitch + (i * 32 + 4 * c) * 2;
-        b0 = *reinterpret_cast<const uint2*>(src);
-        b1 = *reinterpret_cast<const uint2*>(src + 32);
+      const float m0 = pivot(a.m[n][0]), m1 = pivot(a.m[n][1]), M0 = pivot(a.M[n][0]), M1 = pivot(a.M[n][1]);
+#pragma unroll
+      for (int x = 0; x < H; ++x) {
+        a.l[n][0] += ex2(s[x][n][0] - m0) + ex2(s[x][n][2] - m0);
+        a.l[n][1] += ex2(s[x][n][1] - m1) + ex2(s[x][n][3] - m1);
+        const float f0 = lv[x] - M0, f1 = lv[x] - M1;
+        pb[x][n][0] = movmatrix_trans(pack_f16x2(ex2(s[x][n][0] + f0), ex2(s[x][n][1] + f1)));
+        pb[x][n][1] = movmatrix_trans(pack_f16x2(ex2(s[x][n][2] + f0), ex2(s[x][n][3] + f1)));
       }
-      mma_f16(s[n], a0, a1, a2, a3, b0.x, b0.y);
-      mma_f16(s2[n], c0, c1, c2, c3, b1.x, b1.y);
     }
-  }
-  const float lv = log2f(vs);  // -inf for a block of zeros
-  // every member sees slots [0, position]; past them the chain rule decides per token
-  const bool tail = slice + 16 > (p.chain != nullptr ? position + 1 : len);
-  uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+    if (!tail) {
 #pragma unroll
-  for (int n = 0; n < NG; ++n) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * (a.qs[n][e & 1] * ks);
-  }
-  if (tail) {
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int slot = slice + g + (e >> 1) * 8;
-        const int t = p.chain != nullptr ? (chunk * p.width + n * 8 + 2 * c + (e & 1)) / p.groups : 0;
-        if (!sees(slot, len, position, t, chain)) s[n][e] = -INFINITY;
-      }
-    // slots past the row hold anything, NaN codes too: a zero weight must not meet them
-    const int left = len - slice;
-    keep0 = (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
-    keep1 = (2 * c + 8 < left ? 0xffffu : 0u) | (2 * c + 9 < left ? 0xffff0000u : 0u);
-  }
-  bool moves = false;
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      moves = moves || fmaxf(s[n][e], s[n][e + 2]) > fminf(a.m[n][e], a.M[n][e] - lv) + kSlack;
-  if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(s[n][e], s[n][e + 2]);
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float m = fmaxf(a.m[n][e], top), M = fmaxf(a.M[n][e], top + lv);
-        const float fl = ex2(a.m[n][e] - pivot(m)), fo = ex2(a.M[n][e] - pivot(M));
-        a.m[n][e] = m;
-        a.M[n][e] = M;
-        a.l[n][e] *= fl;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          a.o[n][k][e] *= fo;
-          a.o[n][k][e + 2] *= fo;
-        }
-      }
-  }
-  uint32_t pb[NG][2];
-#pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    float w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a.l[n][e & 1] += ex2(s[n][e] - pivot(a.m[n][e & 1]));
-      w[e] = ex2(s[n][e] + lv - pivot(a.M[n][e & 1]));
+      for (int x = 0; x < H; ++x) value_product<D, NG>(a.o, vt, row + 16 * x, half, kPick, kPick, pb[x]);
+      continue;
     }
-    pb[n][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
-    pb[n][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
-  }
-  if (tail && p.chain != nullptr && any_nan<D>(vt, warp, lane)) {
-    // A NaN in a slot that only some members see: their zero weights must not meet it, so each
-    // member's column is kept from a product of its own, over the slots it sees. Never taken on
-    // sound values.
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+    for (int x = 0; x < H; ++x) {
+      const int left = len - slice - 16 * x;
+      // A NaN in a slot that only some members see: their zero weights must not meet it, so each
+      // member's column is kept from a product of its own, over the slots it sees. Never taken on
+      // sound values.
+      if (p.chain != nullptr && left > 0 && any_nan<D>(vt, row - (lane & 15) + 16 * x, lane)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
 #pragma unroll 1
-      for (int col = 0; col < 8 && n * 8 + col < p.width; ++col) {
-        const int t = (chunk * p.width + n * 8 + col) / p.groups;
-        uint32_t k0 = 0u, k1 = 0u;
+          for (int col = 0; col < 8 && n * 8 + col < p.width; ++col) {
+            const int t = (chunk * p.width + n * 8 + col) / p.groups;
+            bool seen[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = slice + 2 * c + (e & 1) + (e >> 1) * 8;
-          if (!sees(slot, len, position, t, chain)) continue;
-          (e < 2 ? k0 : k1) |= (e & 1) ? 0xffff0000u : 0xffffu;
-        }
-        const uint32_t one[1][2] = {{pb[n][0], pb[n][1]}};
-        float o[1][D / 16][4] = {};
-        value_product<D, 1>(o, vt, row, half, k0, k1, one);
-        if (col >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
+            for (int e = 0; e < 4; ++e)
+              seen[e] = sees(slice + 16 * x + 2 * c + (e & 1) + (e >> 1) * 8, len, position, t, chain);
+            const uint32_t one[1][2] = {{pb[x][n][0], pb[x][n][1]}};
+            float o[1][D / 16][4] = {};
+            value_product<D, 1>(o, vt, row + 16 * x, half, pick_slots(seen[0], seen[1]), pick_slots(seen[2], seen[3]), one);
+            if (col >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          (col & 1 ? a.o[n][k][1] : a.o[n][k][0]) += col & 1 ? o[0][k][1] : o[0][k][0];
-          (col & 1 ? a.o[n][k][3] : a.o[n][k][2]) += col & 1 ? o[0][k][3] : o[0][k][2];
-        }
+            for (int k = 0; k < D / 16; ++k) {
+              (col & 1 ? a.o[n][k][1] : a.o[n][k][0]) += col & 1 ? o[0][k][1] : o[0][k][0];
+              (col & 1 ? a.o[n][k][3] : a.o[n][k][2]) += col & 1 ? o[0][k][3] : o[0][k][2];
+            }
+          }
+        continue;
       }
-    return;
+      // slots past the row hold anything, NaN codes too: a zero weight must not meet them
+      value_product<D, NG>(a.o, vt, row + 16 * x, half, pick_slots(2 * c < left, 2 * c + 1 < left),
+                           pick_slots(2 * c + 8 < left, 2 * c + 9 < left), pb[x]);
+    }
   }
-  value_product<D, NG>(a.o, vt, row, half, keep0, keep1, pb);
 }
 
 // Sums the consumer warps' states in warp order, column group by column group: sink(in_chunk, d, O, M,
@@ -432,20 +482,20 @@ __device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, floa
       }
     }
 #pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    if (n * 8 >= members) break;  // uniform
-    if (n > 0) consumers_sync();  // the last group's reads are done
+  for (int pass = 0; pass < 2 * NG; ++pass) {
+    const int n = pass / 2, k0 = pass % 2 * (D / 32);  // column group, half of its dims
+    if (n * 8 >= members) break;                       // uniform
+    if (pass > 0) consumers_sync();                    // the last pass's reads are done
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      float* dst = red_o + (warp * D + 16 * k + 2 * g) * 8 + 2 * c;
-      *reinterpret_cast<float2*>(dst) = make_float2(a.o[n][k][0], a.o[n][k][1]);
-      *reinterpret_cast<float2*>(dst + 8) = make_float2(a.o[n][k][2], a.o[n][k][3]);
+    for (int k = 0; k < D / 32; ++k) {
+      float* dst = red_o + (warp * (D / 2) + 16 * k + 2 * g) * 8 + 2 * c;
+      *reinterpret_cast<float2*>(dst) = make_float2(a.o[n][k0 + k][0], a.o[n][k0 + k][1]);
+      *reinterpret_cast<float2*>(dst + 8) = make_float2(a.o[n][k0 + k][2], a.o[n][k0 + k][3]);
     }
     consumers_sync();
-    // a thread's elements share a column (128 threads cover one or two columns at a time)
 #pragma unroll
-    for (int e0 = 0; e0 < 8 * D; e0 += kWarps * 32) {
-      const int e = e0 + tid, col = e / D, d = e % D, in_chunk = n * 8 + col;
+    for (int e0 = 0; e0 < 8 * (D / 2); e0 += kWarps * 32) {
+      const int e = e0 + tid, col = e / (D / 2), d = e % (D / 2), in_chunk = n * 8 + col;
       if (in_chunk >= members) break;
       float wM[kWarps], wm[kWarps], M = -INFINITY, m = -INFINITY;
 #pragma unroll
@@ -457,10 +507,10 @@ __device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, floa
       float O = 0.f, l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        O += red_o[(w * D + d) * 8 + col] * ex2(wM[w] - pivot(M));
+        O += red_o[(w * (D / 2) + d) * 8 + col] * ex2(wM[w] - pivot(M));
         l += red_stats[(w * NG * 8 + in_chunk) * 3 + 2] * ex2(wm[w] - pivot(m));
       }
-      sink(in_chunk, d, O, M, m, l);
+      sink(in_chunk, k0 * 16 + d, O, M, m, l);
     }
   }
 }
@@ -505,8 +555,8 @@ __device__ __forceinline__ bool load_tile(const Smem<D, NG>& sm, const Params& p
     tma_load_2d(kt + S::kTileBytes, vmap, &sm.full[s], 0, row);
   }
   if (lane < kScales) {
-    const int i = min((j * kTile + (lane % kWarps) * 16) / p.block, p.blocks - 1);
-    const float* src = (lane < kWarps ? p.key_scales : p.value_scales) + static_cast<size_t>(pair) * p.blocks + i;
+    const int i = min((j * kTile + (lane % kSlices) * 16) / p.block, p.blocks - 1);
+    const float* src = (lane < kSlices ? p.key_scales : p.value_scales) + static_cast<size_t>(pair) * p.blocks + i;
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sm.scales + s * kScales + lane)), "l"(src)
                  : "memory");
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[s])) : "memory");
@@ -535,8 +585,8 @@ __device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>&
   }
   __syncwarp();
   const uint32_t kt = smem_u32(sm.ring + s * 2 * S::kTileBytes);
-  const float ks = sm.scales[s * kScales + warp], vs = sm.scales[s * kScales + kWarps + warp];
-  attend_tile<D, NG>(a, p, sm.query, kt, kt + S::kTileBytes, j * kTile, len, position, chain, chunk, ks, vs, warp, lane);
+  attend_tile<D, NG>(a, p, sm.query, sm.scales + s * kScales, kt, kt + S::kTileBytes, j * kTile, len, position, chain,
+                     chunk, warp, lane);
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.empty[s]);
 }

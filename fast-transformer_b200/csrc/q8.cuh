@@ -37,8 +37,16 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
 
 // Two packed e4m3 codes (low 16 bits) to f16x2: exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t h;
+  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(h) : "r"(codes));
+  return h;
+}
+
+// Four packed codes to two f16x2.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
