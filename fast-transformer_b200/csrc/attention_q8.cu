@@ -26,6 +26,8 @@
 //    ragged rows balance. A run of tiles that covers its unit writes the output; others leave
 //    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
 //    calls share nothing.
+#include <type_traits>
+
 #include "q8.cuh"
 
 namespace fb {
@@ -864,7 +866,9 @@ size_t workspace_bytes(const Params& p, int head_dim) {
   return acc_bytes(p, head_dim) + slots * p.width * sizeof(float4);
 }
 
-int shape(Params* p, int batch, int tokens, int q_heads, int kv_heads, int head_dim, int capacity, int block) {
+int shape(Params* p, const fb_q8_cache& cache, int tokens, int q_heads) {
+  const int batch = cache.batch, kv_heads = cache.kv_heads, capacity = cache.capacity;
+  const int head_dim = cache.head_dim, block = cache.block;
   if (batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0) return FB_ERR_ARG;
   if ((head_dim != 64 && head_dim != 128) || !q8::valid_block(block)) return FB_ERR_SHAPE;
   if (q_heads % kv_heads != 0 || batch > kMaxBatch || tokens > capacity) return FB_ERR_SHAPE;
@@ -942,25 +946,36 @@ int cluster_size(const Params& p) {
 }
 
 template <int D, int NG>
-int launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, cudaStream_t stream) {
-  if (!configure<D, NG>()) return FB_ERR_LAUNCH;
+int launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int cluster, cudaStream_t stream) {
   const int units = p.batch * p.kv_heads * p.chunks;
   constexpr int bytes = Smem<D, NG>::kTotal;
-  const int c = cluster_size<D, NG>(p);
-  if (c > 0)
-    return launch_ex(cluster_kernel<D, NG>, dim3(c, units), dim3(kThreads), bytes, stream, c, km, vm, p);
+  if (cluster > 0)
+    return launch_ex(cluster_kernel<D, NG>, dim3(cluster, units), dim3(kThreads), bytes, stream, cluster, km, vm, p);
   const int st = launch_ex(persistent_kernel<D, NG>, dim3(p.ctas), dim3(kThreads), bytes, stream, 1, km, vm, p);
   if (st != FB_OK) return st;
   return launch_ex(merge_kernel<D>, dim3(units, (p.width + 7) / 8), dim3(kMergeThreads), 0, stream, 1, p);
 }
 
-template <int D>
-int launch_groups(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, cudaStream_t stream) {
-  if (p.width <= 8) return launch<D, 1>(km, vm, p, stream);
-  if (p.width <= 16) return launch<D, 2>(km, vm, p, stream);
-  if (p.width <= 24) return launch<D, 3>(km, vm, p, stream);
-  if constexpr (D == 64) return launch<D, 4>(km, vm, p, stream);
-  return FB_ERR_SHAPE;
+// Calls f(head dim, column groups) as compile-time constants.
+template <int D, typename F>
+auto with_groups(const Params& p, F f) {
+  using std::integral_constant;
+  if (p.width <= 8) return f(integral_constant<int, D>(), integral_constant<int, 1>());
+  if (p.width <= 16) return f(integral_constant<int, D>(), integral_constant<int, 2>());
+  if (D == 128 || p.width <= 24) return f(integral_constant<int, D>(), integral_constant<int, 3>());
+  return f(integral_constant<int, D>(), integral_constant<int, D == 64 ? 4 : 3>());
+}
+template <typename F>
+auto with_shape(const Params& p, int head_dim, F f) {
+  return head_dim == 128 ? with_groups<128>(p, f) : with_groups<64>(p, f);
+}
+
+// The cluster size a shape runs with (0: persistent), or an error.
+int plan(const Params& p, int head_dim) {
+  return with_shape(p, head_dim, [&](auto d, auto ng) {
+    constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
+    return configure<D, NG>() ? cluster_size<D, NG>(p) : static_cast<int>(FB_ERR_LAUNCH);
+  });
 }
 
 }  // namespace attn8
@@ -968,42 +983,51 @@ int launch_groups(const CUtensorMap& km, const CUtensorMap& vm, const Params& p,
 
 using namespace fb;
 
-extern "C" size_t fb_attention_q8_workspace(int batch, int tokens, int q_heads, int kv_heads, int head_dim,
-                                            int capacity, int block) {
+extern "C" size_t fb_attention_q8_workspace(const fb_q8_cache* cache, int tokens, int q_heads) {
   attn8::Params p;
-  if (attn8::shape(&p, batch, tokens, q_heads, kv_heads, head_dim, capacity, block) != FB_OK) return 0;
-  return attn8::workspace_bytes(p, head_dim);
+  if (cache == nullptr || attn8::shape(&p, *cache, tokens, q_heads) != FB_OK) return ~size_t(0);
+  return attn8::plan(p, cache->head_dim) > 0 ? 0 : attn8::workspace_bytes(p, cache->head_dim);
 }
 
-extern "C" int fb_attention_q8(const void* q, const void* keys, const void* values, const float* key_scales,
-                               const float* value_scales, const int64_t* position, int per_row, const int64_t* chain,
-                               void* out, void* workspace, size_t workspace_bytes, int batch, int tokens, int q_heads,
-                               int kv_heads, int head_dim, int capacity, int block, float scale, void* stream) {
-  if (!q || !keys || !values || !key_scales || !value_scales || !position || !out || !workspace) return FB_ERR_ARG;
+extern "C" int fb_attention_q8(const void* q, const fb_q8_cache* cache, const int64_t* position, int per_row,
+                               const int64_t* chain, void* out, void* workspace, size_t workspace_bytes, int tokens,
+                               int q_heads, float scale, void* stream) {
+  if (!q || !cache || !position || !out) return FB_ERR_ARG;
+  if (!cache->keys || !cache->values || !cache->key_scales || !cache->value_scales) return FB_ERR_ARG;
   attn8::Params p;
-  int st = attn8::shape(&p, batch, tokens, q_heads, kv_heads, head_dim, capacity, block);
+  int st = attn8::shape(&p, *cache, tokens, q_heads);
   if (st != FB_OK) return st;
   if ((chain == nullptr && tokens != 1) || (chain != nullptr && !per_row)) return FB_ERR_ARG;
-  if (workspace_bytes < attn8::workspace_bytes(p, head_dim)) return FB_ERR_WORKSPACE;
-  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 || (reinterpret_cast<uintptr_t>(q) & 7u) != 0)
-    return FB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) & 7u) != 0) return FB_ERR_ARG;
+  const int head_dim = cache->head_dim;
+  const int cluster = attn8::plan(p, head_dim);
+  if (cluster < 0) return cluster;
+  if (cluster == 0) {
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return FB_ERR_ARG;
+    if (workspace_bytes < attn8::workspace_bytes(p, head_dim)) return FB_ERR_WORKSPACE;
+    p.acc = static_cast<float*>(workspace);
+    p.stats = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + attn8::acc_bytes(p, head_dim));
+  } else {
+    p.acc = nullptr;
+    p.stats = nullptr;
+  }
   p.q = static_cast<const __nv_bfloat16*>(q);
-  p.key_scales = key_scales;
-  p.value_scales = value_scales;
+  p.key_scales = cache->key_scales;
+  p.value_scales = cache->value_scales;
   p.position = position;
   p.chain = chain;
   p.per_row = per_row ? 1 : 0;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.acc = static_cast<float*>(workspace);
-  p.stats = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + attn8::acc_bytes(p, head_dim));
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   p.err = error_word();
-  const uint64_t rows = static_cast<uint64_t>(batch) * kv_heads * capacity;
+  const uint64_t rows = static_cast<uint64_t>(p.batch) * p.kv_heads * p.capacity;
   CUtensorMap km, vm;
-  st = encode_u8_2d(&km, keys, rows, head_dim, attn8::kTile);
+  st = encode_u8_2d(&km, cache->keys, rows, head_dim, attn8::kTile);
   if (st != FB_OK) return st;
-  st = encode_u8_2d(&vm, values, rows, head_dim, attn8::kTile);
+  st = encode_u8_2d(&vm, cache->values, rows, head_dim, attn8::kTile);
   if (st != FB_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return head_dim == 128 ? attn8::launch_groups<128>(km, vm, p, s) : attn8::launch_groups<64>(km, vm, p, s);
+  return attn8::with_shape(p, head_dim, [&](auto d, auto ng) {
+    return attn8::launch<decltype(d)::value, decltype(ng)::value>(km, vm, p, cluster, s);
+  });
 }

@@ -274,12 +274,12 @@ using namespace fb;
 extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, const void* q_weight,
                                          const void* k_weight, float q_eps, float k_eps, const void* cos,
                                          const void* sin, const int64_t* position, const int64_t* phases,
-                                         void* query, void* keys, void* values, float* key_scales,
-                                         float* value_scales, int batch, int tokens, int q_heads, int kv_heads,
-                                         int head_dim, int capacity, int block, int mode, int table, void* stream) {
-  if (!packed || !q_weight || !k_weight || !cos || !sin || !position || !query || !keys || !values || !key_scales ||
-      !value_scales)
-    return FB_ERR_ARG;
+                                         void* query, const fb_q8_cache* cache, int tokens, int q_heads, int mode,
+                                         int table, void* stream) {
+  if (!packed || !q_weight || !k_weight || !cos || !sin || !position || !query || !cache) return FB_ERR_ARG;
+  if (!cache->keys || !cache->values || !cache->key_scales || !cache->value_scales) return FB_ERR_ARG;
+  const int batch = cache->batch, kv_heads = cache->kv_heads, capacity = cache->capacity, head_dim = cache->head_dim;
+  const int block = cache->block;
   if (batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0 || packed_splits < 0)
     return FB_ERR_ARG;
   if (mode < 0 || mode > 2 || (table && mode == 1) || (phases && !table)) return FB_ERR_ARG;
@@ -296,10 +296,10 @@ extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, 
   p.position = position;
   p.phases = phases;
   p.query = static_cast<__nv_bfloat16*>(query);
-  p.keys = static_cast<uint8_t*>(keys);
-  p.values = static_cast<uint8_t*>(values);
-  p.key_scales = key_scales;
-  p.value_scales = value_scales;
+  p.keys = static_cast<uint8_t*>(cache->keys);
+  p.values = static_cast<uint8_t*>(cache->values);
+  p.key_scales = cache->key_scales;
+  p.value_scales = cache->value_scales;
   p.batch = batch;
   p.tokens = tokens;
   p.q_heads = q_heads;

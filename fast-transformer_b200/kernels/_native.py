@@ -47,17 +47,14 @@ _SIGNATURES = {
                                         _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                         _c_int, _c_int, _vp]),
     "fb_qk_norm_rope_append_q8": (_c_int, [_vp, _c_int, _vp, _vp, _c_float, _c_float, _vp, _vp, _vp, _vp, _vp, _vp,
-                                           _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                                           _c_int, _c_int, _vp]),
+                                           _c_int, _c_int, _c_int, _c_int, _vp]),
     "fb_spec_relocate_q8": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
-    "fb_attention_q8_workspace": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
-    "fb_attention_q8": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int,
-                                 _c_int, _c_int, _c_int, _c_int, _c_float, _vp]),
+    "fb_attention_q8_workspace": (_c_size, [_vp, _c_int, _c_int]),
+    "fb_attention_q8": (_c_int, [_vp, _vp, _vp, _c_int, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_float, _vp]),
     "fb_w4_packed_bytes": (_c_size, [_c_int, _c_int, _c_int]),
-    "fb_w4_scale_bytes": (_c_size, [_c_int, _c_int, _c_int]),
-    "fb_w4_pack": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
-    "fb_w4_dequantize": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
-    "fb_linear_w4": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
+    "fb_w4_pack": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "fb_w4_dequantize": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "fb_linear_w4": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
     "fb_rmsnorm": (_c_int, [_vp, _c_i64, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
     "fb_add_rmsnorm": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
     "fb_embed_rmsnorm": (_c_int, [_vp, _vp, _c_i64, _vp, _vp, _vp, _c_int, _c_int, _c_float, _vp]),
@@ -89,6 +86,13 @@ _SIGNATURES = {
 }
 
 
+class Q8Cache(ctypes.Structure):
+    """fb_q8_cache: one layer's 8-bit cache (host struct of device pointers)."""
+
+    _fields_ = [("keys", _vp), ("values", _vp), ("key_scales", _vp), ("value_scales", _vp), ("batch", _c_int),
+                ("kv_heads", _c_int), ("capacity", _c_int), ("head_dim", _c_int), ("block", _c_int)]
+
+
 def _load():
     if not os.path.exists(LIBRARY_PATH):
         raise ImportError(
@@ -111,7 +115,7 @@ def exported_names():
 
 
 #: Kernels each launching entry point enqueues (fb_argmax runs two stages).
-_KERNELS_PER_CALL = {"fb_argmax": 2, "fb_attention_q8": 2}
+_KERNELS_PER_CALL = {"fb_argmax": 2}
 _NON_LAUNCHING = {"fb_device_error"}
 #: Running count of libfastb200 kernels enqueued (or recorded into a graph) by this process.
 launches = 0

@@ -15,7 +15,7 @@ mma.sync partials over a balanced persistent split) and fb_decode_attention_comb
 import torch
 
 from kernels import _native
-from kernels._native import check, lib, ptr, stream
+from kernels._native import check, launch, lib, ptr, stream
 
 _CTAS = {}
 
@@ -120,19 +120,19 @@ def block_attention(query, key, value, position, scale, chain, splits=None):
 
 
 def _attend_q8(query, cache, position, per_row, chain, tokens, q_heads, shape, scale):
-    device = query.device
-    _native.require_device(device, cache.keys, position, chain)
+    device = cache.device
+    if query.device != device or position.device != device or (chain is not None and chain.device != device):
+        raise ValueError(f"8-bit attention takes tensors on the cache's device, {device}")
     assert query.dtype == torch.bfloat16 and query.is_contiguous()
     assert position.dtype == torch.int64 and position.is_contiguous()
-    out = torch.empty(shape, device=device, dtype=torch.bfloat16)
     need = cache.workspace_bytes(tokens, q_heads)
-    if need == 0:
-        raise ValueError(f"attention over {cache.batch} x {cache.kv_heads} x {cache.capacity} slots is too large")
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _native.launch("fb_attention_q8", device, query.data_ptr(), cache.keys.data_ptr(), cache.values.data_ptr(),
-                   cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), position.data_ptr(), per_row,
-                   chain.data_ptr() if chain is not None else None, out.data_ptr(), workspace.data_ptr(), need,
-                   cache.batch, tokens, q_heads, cache.kv_heads, cache.dim, cache.capacity, cache.block, scale)
+    out = query.new_empty(shape)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    launch("fb_attention_q8", device, query.data_ptr(), cache.address, position.data_ptr(), per_row,
+           None if chain is None else chain.data_ptr(), out.data_ptr(), workspace.data_ptr() if need else None, need,
+           tokens, q_heads, scale)
+    if need:
+        _native.launches += 1  # the merge
     return out
 
 
@@ -143,7 +143,7 @@ def decode_attention_q8(query, cache, position, scale):
     assert tokens == 1 and batch == cache.batch and dim == cache.dim and q_heads % cache.kv_heads == 0
     assert position.shape == (1,) or position.shape == (batch,)
     return _attend_q8(query, cache, position, 1 if position.shape[0] > 1 else 0, None, 1, q_heads,
-                      (batch, 1, q_heads, dim), float(scale))
+                      (batch, 1, q_heads, dim), scale)
 
 
 def block_attention_q8(query, cache, position, scale, chain):
@@ -153,4 +153,4 @@ def block_attention_q8(query, cache, position, scale, chain):
     assert 0 < tokens <= cache.capacity and batch == cache.batch and dim == cache.dim
     assert q_heads % cache.kv_heads == 0 and position.shape == (batch,)
     assert chain.shape == (batch,) and chain.dtype == torch.int64 and chain.is_contiguous()
-    return _attend_q8(query, cache, position, 1, chain, tokens, q_heads, (batch, tokens, q_heads, dim), float(scale))
+    return _attend_q8(query, cache, position, 1, chain, tokens, q_heads, (batch, tokens, q_heads, dim), scale)

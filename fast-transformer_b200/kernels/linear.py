@@ -21,7 +21,7 @@ import torch
 from torch.nn import functional as F
 
 from kernels import _native
-from kernels._native import check, lib, ptr, stream
+from kernels._native import check, launch, lib, ptr, stream
 from kernels.merged import Split
 from kernels.quant import Weight4
 
@@ -77,41 +77,49 @@ def project(flat, weight, epilogue=BF16_OUT, splits=None):
     return out
 
 
-def _project4(flat, weight, epilogue):
-    """fb_linear_w4 on [M,K]: the outputs of ``project``."""
-    m, k = flat.shape
-    n = weight.shape[0]
-    if k != weight.shape[1] or flat.dtype != torch.bfloat16 or not 0 < m <= MAX_ROWS:
-        raise ValueError(f"4-bit weights {tuple(weight.shape)} take 1 to {MAX_ROWS} BF16 rows of their width, not "
-                         f"{flat.dtype} {tuple(flat.shape)}")
-    device = flat.device
-    _native.require_device(device, weight.packed)
-    if epilogue == SWIGLU_OUT:
-        if n % 128:
-            raise ValueError(f"SwiGLU weights are 64-row gate/up blocks: {n} rows are not a multiple of 128")
-        out = torch.empty((m, n // 2), device=device, dtype=torch.bfloat16)
-    elif epilogue == SPLITS_OUT:
-        out = torch.empty((1, m, n), device=device, dtype=torch.float32)
-    else:
-        out = torch.empty((m, n), device=device, dtype=torch.float32 if epilogue == FP32_OUT else torch.bfloat16)
-    if flat.data_ptr() % 16:
-        flat = flat.clone()
-    _native.launch("fb_linear_w4", device, flat.data_ptr(), weight.packed.data_ptr(), weight.scales.data_ptr(),
-                   out.data_ptr(), m, n, k, weight.group, FP32_OUT if epilogue == SPLITS_OUT else epilogue)
+def _launch4(x, weight, out, rows, epilogue):
+    """fb_linear_w4 on contiguous x of ``rows`` rows."""
+    device = weight.device
+    if x.device != device:
+        raise ValueError(f"4-bit weights on {device} take inputs of that device, not {x.device}")
+    if x.data_ptr() % 16:
+        x = x.clone()
+    launch("fb_linear_w4", device, x.data_ptr(), weight.packed.data_ptr(), out.data_ptr(), rows, weight.n, weight.k, weight.group,
+           epilogue)
     return out
 
 
+def _refuse4(x, weight):
+    raise ValueError(f"4-bit weights {tuple(weight.shape)} take 1 to {MAX_ROWS} BF16 rows of their width, not {x.dtype} "
+                     f"{tuple(x.shape)}")
+
+
+def _project4(flat, weight, epilogue):
+    """fb_linear_w4 on [M,K]: the outputs of ``project``."""
+    m, n = flat.shape[0], weight.n
+    if flat.shape[1] != weight.k or flat.dtype != torch.bfloat16 or not 0 < m <= MAX_ROWS:
+        _refuse4(flat, weight)
+    if epilogue == SWIGLU_OUT:
+        if n % 128:
+            raise ValueError(f"SwiGLU weights are 64-row gate/up blocks: {n} rows are not a multiple of 128")
+        out = flat.new_empty((m, n // 2))
+    elif epilogue == BF16_OUT:
+        out = flat.new_empty((m, n))
+    else:
+        out = flat.new_empty((1, m, n) if epilogue == SPLITS_OUT else (m, n), dtype=torch.float32)
+    return _launch4(flat.contiguous(), weight, out, m, FP32_OUT if epilogue == SPLITS_OUT else epilogue)
+
+
 def _linear4(x, weight):
-    n, k = weight.shape
-    if x.shape[-1] != k or x.dtype != torch.bfloat16:
-        raise ValueError(f"4-bit weights {tuple(weight.shape)} take BF16 [..., {k}], not {x.dtype} {tuple(x.shape)}")
+    shape, k = x.shape, weight.k
+    if shape[-1] != k or x.dtype != torch.bfloat16:
+        _refuse4(x, weight)
     rows = x.numel() // k
-    if rows == 0:
-        return x.new_empty((*x.shape[:-1], n))
     if rows > MAX_ROWS:
         _native.require_device(weight.device, x)
         return F.linear(x, weight.dequantized())
-    return _project4(x.reshape(rows, k).contiguous(), weight, BF16_OUT).view(*x.shape[:-1], n)
+    out = x.new_empty((*shape[:-1], weight.n))
+    return _launch4(x if x.is_contiguous() else x.contiguous(), weight, out, rows, BF16_OUT) if rows else out
 
 
 def linear(x, weight, split_ok=False):

@@ -59,10 +59,10 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, cache, q_heads,
     and sin are whole tables of at least ``cache.capacity`` rows, read at the device-side position.
     Rows at a negative position get nothing appended."""
     split = isinstance(packed, Split)
-    data, splits, _, shape = source(packed)
-    batch, kv_heads, capacity, dim = cache.batch, cache.kv_heads, cache.capacity, cache.dim
+    data, splits = (packed.partial, packed.splits) if split else (packed, 0)
+    batch, kv_heads, capacity, dim, device = cache.batch, cache.kv_heads, cache.capacity, cache.dim, cache.device
+    shape = packed.shape
     tokens = shape[1]
-    device = data.device
     assert data.dtype == (torch.float32 if split else torch.bfloat16) and data.is_contiguous()
     assert shape == (batch, tokens, (q_heads + 2 * kv_heads) * dim) and q_heads > 0
     assert 0 < tokens <= capacity
@@ -80,13 +80,11 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, cache, q_heads,
     q_weight, k_weight = q_norm.weight, k_norm.weight
     assert q_weight.dtype == k_weight.dtype == torch.bfloat16 and q_weight.numel() == k_weight.numel() == dim
     assert q_weight.is_contiguous() and k_weight.is_contiguous()
-    _native.require_device(device, cache.keys, cos, sin, position, phases, q_weight, k_weight)
-    query = torch.empty((batch, tokens, q_heads, dim), device=device, dtype=torch.bfloat16)
+    _native.require_device(device, data, cos, sin, position, phases, q_weight, k_weight)
+    query = cos.new_empty((batch, tokens, q_heads, dim))
     _native.launch(
-        "fb_qk_norm_rope_append_q8", device, data.data_ptr(), splits if split else 0, q_weight.data_ptr(),
-        k_weight.data_ptr(), q_norm.variance_epsilon, k_norm.variance_epsilon, cos.data_ptr(), sin.data_ptr(),
-        position.data_ptr(), phases.data_ptr() if phases is not None else None, query.data_ptr(),
-        cache.keys.data_ptr(), cache.values.data_ptr(), cache.key_scales.data_ptr(), cache.value_scales.data_ptr(),
-        batch, tokens, q_heads, kv_heads, dim, capacity, cache.block, 1 if prefill else 2 if rows else 0,
-        1 if whole else 0)
+        "fb_qk_norm_rope_append_q8", device, data.data_ptr(), splits, q_weight.data_ptr(), k_weight.data_ptr(),
+        q_norm.variance_epsilon, k_norm.variance_epsilon, cos.data_ptr(), sin.data_ptr(), position.data_ptr(),
+        None if phases is None else phases.data_ptr(), query.data_ptr(), cache.address, tokens, q_heads,
+        1 if prefill else 2 if rows else 0, 1 if whole else 0)
     return query.transpose(1, 2)

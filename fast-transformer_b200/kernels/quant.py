@@ -8,6 +8,8 @@ columns, laid out once for ``kernels.linear.linear`` and ``swiglu_linear``, whic
 place of a tensor. The reference has neither: its cache and weights are bf16.
 """
 
+import ctypes
+
 import torch
 
 from kernels import _native
@@ -27,7 +29,7 @@ class QuantCache:
     and the append updates in place."""
 
     __slots__ = ("_keys", "_values", "_key_scales", "_value_scales", "block", "batch", "kv_heads", "capacity", "dim",
-                 "device", "_workspace")
+                 "device", "_struct", "address", "_workspace")
 
     def __init__(self, keys, values, key_scales, value_scales, block=64):
         assert block in BLOCKS
@@ -45,6 +47,9 @@ class QuantCache:
         self._key_scales, self._value_scales = key_scales, value_scales
         self.block, self.device = block, keys.device
         self.batch, self.kv_heads, self.capacity, self.dim = batch, kv_heads, capacity, dim
+        self._struct = _native.Q8Cache(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(),
+                                       value_scales.data_ptr(), batch, kv_heads, capacity, dim, block)
+        self.address = ctypes.addressof(self._struct)  # fb_q8_cache*
         self._workspace = {}
 
     @classmethod
@@ -71,36 +76,40 @@ class QuantCache:
         return expand(self._keys, self._key_scales), expand(self._values, self._value_scales)
 
     def workspace_bytes(self, tokens, q_heads):
-        """Bytes an attention call of this shape needs (fixed per shape and device)."""
+        """Bytes an attention call of this shape needs (0: none; fixed per shape and device)."""
         key = (tokens, q_heads)
-        if key not in self._workspace:
+        need = self._workspace.get(key)
+        if need is None:
             with torch.cuda.device(self.device):
-                self._workspace[key] = int(lib.fb_attention_q8_workspace(
-                    self.batch, tokens, q_heads, self.kv_heads, self.dim, self.capacity, self.block))
-        return self._workspace[key]
+                need = int(lib.fb_attention_q8_workspace(self.address, tokens, q_heads))
+            if need == ctypes.c_size_t(-1).value:
+                raise ValueError(f"8-bit attention of {tokens} x {q_heads} queries over a cache of {self.batch} x "
+                                 f"{self.kv_heads} x {self.capacity} slots is not supported")
+            self._workspace[key] = need
+        return need
 
 
 class Weight4:
-    """A projection's [N, K] weights in 4 bits: ``packed`` codes and ``scales`` in the kernel's layout,
-    one bf16 scale per row and ``group`` columns. Made by ``pack_weight4`` or ``quantize_weight4``."""
+    """A projection's [N, K] weights in 4 bits: ``packed`` holds the codes and one bf16 scale per row and
+    ``group`` columns in the kernel's layout. Made by ``pack_weight4`` or ``quantize_weight4``."""
 
-    __slots__ = ("packed", "scales", "shape", "group", "device")
+    __slots__ = ("packed", "shape", "n", "k", "group", "device")
 
-    def __init__(self, packed, scales, shape, group):
-        self.packed, self.scales = packed, scales
+    def __init__(self, packed, shape, group):
+        self.packed = packed
         self.shape, self.group, self.device = torch.Size(shape), group, packed.device
+        self.n, self.k = self.shape
 
     @property
     def nbytes(self):
         """Bytes one product reads of it."""
-        return self.packed.numel() + self.scales.numel() * 4
+        return self.packed.numel()
 
     def dequantized(self):
         """bf16 [N, K]: code * scale, rounded once (fb_w4_dequantize)."""
         n, k = self.shape
         out = torch.empty((n, k), dtype=torch.bfloat16, device=self.device)
-        _native.launch("fb_w4_dequantize", self.device, self.packed.data_ptr(), self.scales.data_ptr(), out.data_ptr(),
-                       n, k, self.group)
+        _native.launch("fb_w4_dequantize", self.device, self.packed.data_ptr(), out.data_ptr(), n, k, self.group)
         return out
 
 
@@ -127,12 +136,10 @@ def pack_weight4(codes, scales):
         raise ValueError("4-bit codes lie in -8..7")
     codes, scales = codes.contiguous(), scales.contiguous()
     packed = torch.empty(int(lib.fb_w4_packed_bytes(n, k, group)), dtype=torch.uint8, device=codes.device)
-    packed_scales = torch.empty(int(lib.fb_w4_scale_bytes(n, k, group)) // 4, dtype=torch.int32, device=codes.device)
-    _native.launch("fb_w4_pack", codes.device, codes.data_ptr(), scales.data_ptr(), packed.data_ptr(),
-                   packed_scales.data_ptr(), n, k, group)
+    _native.launch("fb_w4_pack", codes.device, codes.data_ptr(), scales.data_ptr(), packed.data_ptr(), n, k, group)
     # a product may read its weights before the kernel ahead of it ends: that must not be this one
     torch.cuda.current_stream(codes.device).synchronize()
-    return Weight4(packed, packed_scales, (n, k), group)
+    return Weight4(packed, (n, k), group)
 
 
 def quantize_weight4(weight, group=128):

@@ -167,8 +167,9 @@ int fb_qk_norm_rope_append(const void* packed, int packed_splits, const void* q_
                            int table, void* stream);
 
 /* ------------------------------------------------------------------------------------
- * The 8-bit KV cache (no counterpart in the reference, whose cache is bf16).
- *   keys, values             e4m3 codes [B, Hkv, C, D] (one layer), 16-byte aligned
+ * The 8-bit KV cache (no counterpart in the reference, whose cache is bf16): one layer's, described
+ * by a host struct of device pointers.
+ *   keys, values             e4m3 codes [B, Hkv, C, D], 16-byte aligned; D in {64, 128}
  *   key_scales, value_scales fp32 [B, Hkv, ceil(C / block)]; block in {16, 32, 64} slots
  *   the value of slot c is code[c] * scale[c / block]
  * The attention takes any scales >= 0; the append writes powers of two. A row whose position is
@@ -185,13 +186,19 @@ int fb_qk_norm_rope_append(const void* packed, int packed_splits, const void* q_
  * fb_spec_relocate_q8: fb_spec_relocate for a store [planes, B, Hkv, C, D] with scales [planes, B,
  *   Hkv, ceil(C / block)]: move_to becomes its block's newest slot, by the append's rule.
  * ---------------------------------------------------------------------------------- */
+typedef struct fb_q8_cache {
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+  int batch, kv_heads, capacity, head_dim, block;
+} fb_q8_cache;
+
 int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, const void* q_weight,
                               const void* k_weight, float q_eps, float k_eps, const void* cos,
                               const void* sin, const int64_t* position, const int64_t* phases,
-                              void* query, void* keys, void* values, float* key_scales,
-                              float* value_scales, int batch, int tokens, int q_heads, int kv_heads,
-                              int head_dim, int capacity, int block, int mode, int table,
-                              void* stream);
+                              void* query, const fb_q8_cache* cache, int tokens, int q_heads,
+                              int mode, int table, void* stream);
 int fb_spec_relocate_q8(void* store, float* scales, int planes, int batch, int kv_heads, int capacity,
                         int head_dim, int block, const int64_t* move_from, const int64_t* move_to,
                         void* stream);
@@ -199,41 +206,37 @@ int fb_spec_relocate_q8(void* store, float* scales, int planes, int batch, int k
 /* Attention over the 8-bit cache: one token per row (chain NULL, tokens 1; position [1] or, with
  * per_row, [B]) or a verify block (chain int64 [B], position [B], per_row 1; the mask rule of
  * fb_verify_attention).
- *   q   bf16 [B, T, Hq, D], 8-byte aligned; out bf16 [B, T, Hq, D]; D in {64, 128}; any Hq / Hkv
- *   workspace: fb_attention_q8_workspace() bytes, 16-byte aligned, any contents; calls that overlap
- *   on the GPU need one each. B <= 1024, B * Hkv * C < 2^31.
+ *   q   bf16 [B, T, Hq, D], 8-byte aligned; out bf16 [B, T, Hq, D]; any Hq / Hkv
+ *   workspace: fb_attention_q8_workspace() bytes (it reads the cache's sizes, not its pointers; 0:
+ *   the shape runs without, workspace may be NULL; (size_t)-1: the shape is not supported), 16-byte
+ *   aligned, any contents; calls that overlap on the GPU need one each.
+ *   B <= 1024, B * Hkv * C < 2^31.
  * fp32 scores, sums and accumulation; P in f16 for the value product. Everything is read after
  * the dependency wait: any kernel may have written the cache or the position just before. */
-size_t fb_attention_q8_workspace(int batch, int tokens, int q_heads, int kv_heads, int head_dim,
-                                 int capacity, int block);
-int fb_attention_q8(const void* q, const void* keys, const void* values, const float* key_scales,
-                    const float* value_scales, const int64_t* position, int per_row,
+size_t fb_attention_q8_workspace(const fb_q8_cache* cache, int tokens, int q_heads);
+int fb_attention_q8(const void* q, const fb_q8_cache* cache, const int64_t* position, int per_row,
                     const int64_t* chain, void* out, void* workspace, size_t workspace_bytes,
-                    int batch, int tokens, int q_heads, int kv_heads, int head_dim, int capacity,
-                    int block, float scale, void* stream);
+                    int tokens, int q_heads, float scale, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Projections with 4-bit weights (no counterpart in the reference): y = x @ W^T,
  * W[n, k] = code[n, k] * scale[n, k / group], codes -8..7, group in {32, 64, 128}, K % group == 0,
  * N % 8 == 0.
  * fb_w4_pack lays codes int8 [N, K] and scales bf16 [N, K / group] out once, into packed
- *   (fb_w4_packed_bytes(), 16-byte aligned) and packed_scales (fb_w4_scale_bytes()); codes outside
- *   -8..7 keep their low four bits.
+ *   (fb_w4_packed_bytes(), 16-byte aligned); codes outside -8..7 keep their low four bits.
  * fb_linear_w4: x bf16 [M, K] (M <= 64, 16-byte aligned); fp32 accumulation of the exact products, one rounding.
  *   epilogue 0: out bf16 [M, N]   1: out fp32 [M, N]   2: SwiGLU on rows interleaved in 64-row
  *   gate/up blocks as for fb_linear (N % 128 == 0): out bf16 [M, N / 2].
- *   The packed weights and scales may be read before the wait on the previous kernel, like
+ *   The packed weights may be read before the wait on the previous kernel, like
  *   fb_linear's: that kernel must not write them.
  * fb_w4_dequantize: the weights as bf16 [N, K] (code * scale rounded once), for library products.
  * ---------------------------------------------------------------------------------- */
 size_t fb_w4_packed_bytes(int n, int k, int group);
-size_t fb_w4_scale_bytes(int n, int k, int group);
-int fb_w4_pack(const int8_t* codes, const void* scales, void* packed, void* packed_scales, int n, int k,
-               int group, void* stream);
-int fb_w4_dequantize(const void* packed, const void* packed_scales, void* out, int n, int k, int group,
-                     void* stream);
-int fb_linear_w4(const void* x, const void* packed, const void* packed_scales, void* out, int m, int n,
-                 int k, int group, int epilogue, void* stream);
+int fb_w4_pack(const int8_t* codes, const void* scales, void* packed, int n, int k, int group,
+               void* stream);
+int fb_w4_dequantize(const void* packed, void* out, int n, int k, int group, void* stream);
+int fb_linear_w4(const void* x, const void* packed, void* out, int m, int n, int k, int group,
+                 int epilogue, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * RMSNorm family. Replace engine/kernels/rmsnorm.py:
