@@ -13,9 +13,15 @@
 //
 // A block has one owner CTA: it holds every new value of the block in registers, reduces the
 // largest magnitude through shared memory, and is the only reader and writer of the block's
-// codes and scale. No atomics. Q heads run in CTAs of their own, a warp per (token, head).
+// codes and scale. No atomics. Q heads run in CTAs of their own, a warp per token and run of heads.
+//
+// A prompt is bound by bytes (the packed projection in, Q and the codes out) and close behind by
+// instructions: a head's D values lie on D / 8 lanes, four dims of each half, so that RoPE's partners
+// meet in a lane (no shuffles but the norm's), and a warp issues all the loads of its rows before it
+// uses one. A decode step is bound by latency.
+#include <initializer_list>
+
 #include "q8.cuh"
-#include "rope_math.cuh"
 
 namespace fb {
 namespace q8 {
@@ -23,7 +29,7 @@ namespace q8 {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlock = 64;
-constexpr int kPerWarp = kMaxBlock / kWarps;  // slots of a block a warp holds
+constexpr int kE = 8;  // values of a lane
 
 struct AppendParams {
   const void* packed;
@@ -40,9 +46,11 @@ struct AppendParams {
   uint8_t* values;
   float* key_scales;
   float* value_scales;
-  int batch, tokens, q_heads, kv_heads, capacity, block, blocks, mode, table;
-  int query_ctas;      // CTAs [0, query_ctas) do Q heads
-  int touched;         // cache blocks a row's tokens can touch
+  int batch, tokens, q_heads, kv_heads, capacity, block, block_shift, blocks, mode, table;
+  int query_ctas;   // CTAs [0, query_ctas) do Q heads
+  int query_heads;  // of a warp's token
+  int runs;         // warps of a token: ceil(q_heads / query_heads)
+  int touched;      // cache blocks a row's tokens can touch
   unsigned* err;
 };
 
@@ -65,99 +73,198 @@ __device__ __forceinline__ long long phase_row(const AppendParams& p, int b, int
   return phase;
 }
 
-// RMSNorm + RoPE of one head on a warp, lane l holding dims [l*E, l*E + E): in place, in fp32.
+// How a row of D values lies on a warp: D / 8 lanes, 32 / that many rows side by side; a lane holds dims
+// d0 .. d0 + 3 and D / 2 + d0 .. D / 2 + d0 + 3, d0 = 4 (lane % kLanes).
 template <int D>
-__device__ __forceinline__ void norm_rope_fp32(float (&x)[D / 32], const float (&gain)[D / 32], float eps,
-                                               const float (&cs)[D / 32], const float (&sn)[D / 32], int lane) {
-  constexpr int E = D / 32;
+struct Lanes {
+  static constexpr int kLanes = D / kE, kRows = 32 / kLanes;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[kE]) {
+  x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
+  x[4] = bf16_lo(w.z), x[5] = bf16_hi(w.z), x[6] = bf16_lo(w.w), x[7] = bf16_hi(w.w);
+}
+
+// A lane's eight bf16 values of a row, src at its d0.
+template <int D>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* src) {
+  const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + D / 2);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// A lane's values of a row of the packed projection, `off` its first element: bf16, or fp32 split partials
+// summed in split order and rounded to bf16 (the projection's own rounding).
+template <int D, bool kSplit>
+__device__ __forceinline__ void load_packed8(const AppendParams& p, size_t off, size_t split_stride, float (&x)[kE]) {
+  if constexpr (!kSplit) {
+    unpack8(load8<D>(static_cast<const __nv_bfloat16*>(p.packed) + off), x);
+    return;
+  }
+  const float* src = static_cast<const float*>(p.packed) + off;
+  constexpr int kBatch = 4;  // slabs in flight before their in-order adds
+  for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+    float4 y[kBatch][2];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (s0 + j < p.splits) {
+        y[j][0] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + j) * split_stride));
+        y[j][1] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + j) * split_stride + D / 2));
+      }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (s0 + j < p.splits) {
+        const float v[kE] = {y[j][0].x, y[j][0].y, y[j][0].z, y[j][0].w, y[j][1].x, y[j][1].y, y[j][1].z, y[j][1].w};
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[e] = s0 + j == 0 ? v[e] : x[e] + v[e];
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < kE; ++e) x[e] = bf16_round(x[e]);
+}
+
+// RMSNorm + RoPE of the rows on a warp, in place, in fp32: w = x * inv * gain, out = w cos + rot(w) sin.
+template <int D>
+__device__ __forceinline__ void norm_rope_fp32(float (&x)[kE], const uint4& gain, float eps, const uint4& cos,
+                                               const uint4& sin, int lane) {
+  constexpr int kLanes = Lanes<D>::kLanes;
+  float g[kE], cs[kE], sn[kE];
+  unpack8(gain, g);
+  unpack8(cos, cs);
+  unpack8(sin, sn);
   float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-  const float inv = __frsqrt_rn(warp_sum(ss) / static_cast<float>(D) + eps);
+  for (int e = 0; e < kE; ++e) ss += x[e] * x[e];
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = x[e] * inv * gain[e];
+  for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = __frsqrt_rn(ss / static_cast<float>(D) + eps);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float partner = __shfl_xor_sync(0xffffffffu, x[e], 16);
-    x[e] = x[e] * cs[e] + (lane < 16 ? -partner : partner) * sn[e];
+  for (int e = 0; e < 4; ++e) {
+    const float low = x[e] * inv * g[e], high = x[e + 4] * inv * g[e + 4];
+    x[e] = low * cs[e] - high * sn[e];
+    x[e + 4] = high * cs[e + 4] + low * sn[e + 4];
   }
 }
 
-template <int E>
-__device__ __forceinline__ void store_codes(uint8_t* dst, const float (&x)[E], float inverse) {
-  const uint32_t lo = to_e4m3x2(x[0] * inverse, x[1] * inverse);
-  if constexpr (E == 4)
-    *reinterpret_cast<uint32_t*>(dst) = lo | (to_e4m3x2(x[2] * inverse, x[3] * inverse) << 16);
-  else
-    *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(lo);
+// Four values times `factor` to packed codes; kChecked: anything that is not finite to the NaN code.
+template <bool kChecked>
+__device__ __forceinline__ uint32_t codes4(const float* x, float factor) {
+  if constexpr (kChecked)
+    return to_e4m3x2(x[0] * factor, x[1] * factor) | (to_e4m3x2(x[2] * factor, x[3] * factor) << 16);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * factor, x[1] * factor), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * factor, x[3] * factor), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
 }
 
-template <int E>
-__device__ __forceinline__ void load_codes(const uint8_t* src, float (&x)[E]) {
-  if constexpr (E == 4) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
+template <int D, bool kChecked>
+__device__ __forceinline__ void store_codes8(uint8_t* dst, const float (&x)[kE], float factor) {
+  *reinterpret_cast<uint32_t*>(dst) = codes4<kChecked>(x, factor);
+  *reinterpret_cast<uint32_t*>(dst + D / 2) = codes4<kChecked>(x + 4, factor);
+}
+
+template <int D>
+__device__ __forceinline__ void load_codes8(const uint8_t* src, float (&x)[kE]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * (D / 2));
     const float2 a = e4m3x2_to_float2(w & 0xffffu), b = e4m3x2_to_float2(w >> 16);
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-  } else {
-    const float2 a = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(src));
-    x[0] = a.x, x[1] = a.y;
+    x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = b.x, x[4 * i + 3] = b.y;
   }
 }
 
-// Largest finite magnitude of E values (NaN and infinities do not set a scale).
-template <int E>
-__device__ __forceinline__ float finite_max(const float (&x)[E], float so_far) {
+constexpr uint32_t kInfinity = 0x7f800000u;  // bits: anything from here on is not finite
+
+// Bits of the largest magnitude (they order as the magnitudes do; NaN above infinity above all).
+__device__ __forceinline__ uint32_t max_bits(const float (&x)[kE], uint32_t so_far) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
+  for (int e = 0; e < kE; ++e) so_far = max(so_far, __float_as_uint(x[e]) & 0x7fffffffu);
+  return so_far;
+}
+
+// Largest finite magnitude (NaN and infinities do not set a scale).
+__device__ __forceinline__ float finite_max(const float (&x)[kE], float so_far) {
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
     const float a = fabsf(x[e]);
     so_far = a < INFINITY ? fmaxf(so_far, a) : so_far;
   }
   return so_far;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
-  constexpr int E = D / 32;
+// What a launch does: both parts (a decode step: one launch), or, for a prompt, Q heads and blocks in
+// launches of their own, each at the occupancy that its registers allow (one launch of both: 75 us
+// for 8192 tokens of 32 + 8 heads of 128, two: 55 us).
+enum Part : int { kBoth = 0, kQueries = 1, kBlocks = 2 };
+
+template <int D, bool kSplit, int kPart>
+__global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart == kQueries ? 4 : 3) append_kernel(const AppendParams p) {
+  constexpr int kLanes = Lanes<D>::kLanes, kRows = Lanes<D>::kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int d0 = lane * E;
+  const int sub = lane / kLanes, d0 = lane % kLanes * 4;
   const int width = (p.q_heads + 2 * p.kv_heads) * D;
   const size_t split_stride = static_cast<size_t>(p.batch) * p.tokens * width;
   pdl_wait();
   pdl_trigger();
 
-  if (static_cast<int>(blockIdx.x) < p.query_ctas) {
-    const long long item = static_cast<long long>(blockIdx.x) * kWarps + warp;
-    const long long rows = static_cast<long long>(p.batch) * p.tokens;
-    if (item >= rows * p.q_heads) return;
-    const int row = static_cast<int>(item / p.q_heads), head = static_cast<int>(item % p.q_heads);
-    const int b = row / p.tokens, t = row % p.tokens;
-    float x[E], gain[E], cs[E], sn[E];
-    rope::load_packed_values<E, 8>(p.packed, p.splits, static_cast<size_t>(row) * width + head * D + d0, split_stride, x);
-    rope::load_bf16<E>(p.q_weight + d0, gain);
+  if (kPart != kBlocks && static_cast<int>(blockIdx.x) < p.query_ctas) {
+    // ---- query_heads heads of one token, kRows side by side ----
+    const unsigned item = blockIdx.x * kWarps + warp;  // < 2^31 + kWarps
+    const unsigned nth_row = item / p.runs;
+    const int head0 = static_cast<int>(item - nth_row * p.runs) * p.query_heads;
+    if (nth_row >= static_cast<unsigned>(p.batch * p.tokens)) return;
+    const int row = static_cast<int>(nth_row), b = row / p.tokens, t = row - b * p.tokens;
+    const int heads = min(p.query_heads, p.q_heads - head0);
+    constexpr int kMost = 4;  // loads in flight
+    const size_t in = static_cast<size_t>(row) * width + head0 * D + d0;
+    __nv_bfloat16* out = p.query + (static_cast<size_t>(row) * p.q_heads + head0) * D + d0;
     const size_t phase = static_cast<size_t>(phase_row(p, b, t, first_slot(p, b))) * D + d0;
-    rope::load_bf16<E>(p.cos + phase, cs);
-    rope::load_bf16<E>(p.sin + phase, sn);
-    norm_rope_fp32<D>(x, gain, p.q_eps, cs, sn, lane);
-    __nv_bfloat16* dst = p.query + (static_cast<size_t>(row) * p.q_heads + head) * D + d0;
-    if constexpr (E == 4)
+    const uint4 gain = load8<D>(p.q_weight + d0), cos = load8<D>(p.cos + phase), sin = load8<D>(p.sin + phase);
+    // rows of lanes past the last head repeat it and store nothing
+    auto finish = [&](float (&x)[kE], int h) {
+      norm_rope_fp32<D>(x, gain, p.q_eps, cos, sin, lane);
+      if (h >= heads) return;
+      __nv_bfloat16* dst = out + static_cast<size_t>(h) * D;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-    else
-      *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(x[0], x[1]);
+      *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    };
+    if constexpr (kSplit) {
+      for (int h = sub; h - sub < heads; h += kRows) {
+        float x[kE];
+        load_packed8<D, true>(p, in + static_cast<size_t>(min(h, heads - 1)) * D, split_stride, x);
+        finish(x, h);
+      }
+    } else {
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.packed) + in;
+      for (int h0 = 0; h0 < heads; h0 += kMost * kRows) {
+        uint4 raw[kMost];
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+          raw[i] = load8<D>(src + static_cast<size_t>(min(h0 + i * kRows + sub, heads - 1)) * D);
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+          if (h0 + i * kRows >= heads) break;  // warp-uniform
+          float x[kE];
+          unpack8(raw[i], x);
+          finish(x, h0 + i * kRows + sub);
+        }
+      }
+    }
     return;
   }
+  if (kPart == kQueries) return;
 
   // ---- one cache block of one (row, KV head, K or V) ----
-  __shared__ float s_largest[kWarps];
-  int item = blockIdx.x - p.query_ctas;
+  __shared__ uint32_t s_largest[kWarps];
+  __shared__ float s_finite[kWarps];
+  int item = blockIdx.x - (kPart == kBlocks ? 0 : p.query_ctas);
   const int nth = item % p.touched;
   item /= p.touched;
   const bool is_value = item & 1;
   const int pair = item >> 1;
-  const int b = pair / p.kv_heads, h = pair % p.kv_heads;
+  const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
   const long long start = first_slot(p, b);
   if (start < 0) return;  // whole CTA
-  const long long at = start / p.block + nth;  // block index
-  const long long low = at * p.block;
+  const long long at = (start >> p.block_shift) + nth;  // block index
+  const long long low = at << p.block_shift;
   if (low >= p.capacity || low >= start + p.tokens) {
     if (low < start + p.tokens && threadIdx.x == 0) raise_error(p.err, kErrBadShape);  // tokens past the cache
     return;
@@ -167,52 +274,80 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
   const bool joins = start > low;  // the block holds earlier slots
   const float before = joins ? *scale_at : 0.f;
 
+  // this lane's slots of the block: warp * kRows + sub, and every kWarps * kRows from there
   const int head = p.q_heads + (is_value ? p.kv_heads : 0) + h;
-  float gain[E];
-  if (!is_value) rope::load_bf16<E>(p.k_weight + d0, gain);
-  float x[kPerWarp][E];
-  float largest = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPerWarp; ++i) {
-    const int offset = warp + i * kWarps;
-    const long long t = low + offset - start;
-    if (offset >= p.block || t < 0 || t >= p.tokens) continue;  // warp-uniform
-    if (low + offset >= p.capacity) {
-      if (lane == 0) raise_error(p.err, kErrBadShape);
-      continue;
-    }
-    const size_t row = static_cast<size_t>(b) * p.tokens + t;
-    rope::load_packed_values<E, 2>(p.packed, p.splits, row * width + head * D + d0, split_stride, x[i]);
-    if (!is_value) {
-      float cs[E], sn[E];
-      const size_t phase = static_cast<size_t>(phase_row(p, b, static_cast<int>(t), start)) * D + d0;
-      rope::load_bf16<E>(p.cos + phase, cs);
-      rope::load_bf16<E>(p.sin + phase, sn);
-      norm_rope_fp32<D>(x[i], gain, p.k_eps, cs, sn, lane);
-    }
-    largest = finite_max<E>(x[i], largest);
+  constexpr int kStep = kWarps * kRows, kSlots = kMaxBlock / kStep;
+  const int slot0 = warp * kRows + sub;
+  // slots that get a token
+  const int from = static_cast<int>(start > low ? start - low : 0);
+  long long last = start + p.tokens - low;
+  if (last > p.capacity - low) {
+    if (threadIdx.x == 0) raise_error(p.err, kErrBadShape);  // tokens past the cache
+    last = p.capacity - low;
   }
-  largest = warp_max(largest);
-  if (lane == 0) s_largest[warp] = largest;
+  const int to = static_cast<int>(last < p.block ? last : p.block);
+  float x[kSlots][kE];
+  uint4 cos[kSlots], sin[kSlots], gain;
+  if (!is_value) gain = load8<D>(p.k_weight + d0);
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    const int slot = slot0 + i * kStep;
+    const bool fresh = slot >= from && slot < to;
+    if (fresh) {
+      const int t = static_cast<int>(low + slot - start);
+      load_packed8<D, kSplit>(p, (static_cast<size_t>(b) * p.tokens + t) * width + head * D + d0, split_stride, x[i]);
+      if (!is_value) {
+        const size_t phase = static_cast<size_t>(phase_row(p, b, t, start)) * D + d0;
+        cos[i] = load8<D>(p.cos + phase);
+        sin[i] = load8<D>(p.sin + phase);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) x[i][e] = 0.f;
+      cos[i] = sin[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    if (!is_value) norm_rope_fp32<D>(x[i], gain, p.k_eps, cos[i], sin[i], lane);  // zeros stay zeros
+    bits = max_bits(x[i], bits);
+  }
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  if (lane == 0) s_largest[warp] = bits;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) largest = fmaxf(largest, s_largest[w]);
+  for (int w = 0; w < kWarps; ++w) bits = max(bits, s_largest[w]);
+  float largest = __uint_as_float(bits);
+  const bool sound = bits < kInfinity;
+  if (!sound) {  // some value is not finite (the whole CTA agrees): the largest of the others
+    largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) largest = finite_max(x[i], largest);
+    largest = warp_max(largest);
+    if (lane == 0) s_finite[warp] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) largest = fmaxf(largest, s_finite[w]);
+  }
   const float after = fmaxf(least_scale(largest), before);
   const float inverse = 1.f / after;
   if (joins && after > before) {
     const float ratio = before * inverse;
-    for (int offset = warp; offset < p.block && low + offset < start; offset += kWarps) {
-      float old[E];
-      load_codes<E>(codes + static_cast<size_t>(offset) * D, old);
-      store_codes<E>(codes + static_cast<size_t>(offset) * D, old, ratio);
+    for (int slot = slot0; slot < from; slot += kStep) {
+      float old[kE];
+      load_codes8<D>(codes + static_cast<size_t>(slot) * D, old);
+      store_codes8<D, true>(codes + static_cast<size_t>(slot) * D, old, ratio);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kPerWarp; ++i) {
-    const int offset = warp + i * kWarps;
-    const long long t = low + offset - start;
-    if (offset >= p.block || t < 0 || t >= p.tokens || low + offset >= p.capacity) continue;
-    store_codes<E>(codes + static_cast<size_t>(offset) * D, x[i], inverse);
+  for (int i = 0; i < kSlots; ++i) {
+    const int slot = slot0 + i * kStep;
+    if (slot < from || slot >= to) continue;
+    if (sound)
+      store_codes8<D, false>(codes + static_cast<size_t>(slot) * D, x[i], inverse);
+    else
+      store_codes8<D, true>(codes + static_cast<size_t>(slot) * D, x[i], inverse);
   }
   if (threadIdx.x == 0) *scale_at = after;
 }
@@ -226,11 +361,11 @@ __global__ void __launch_bounds__(128) relocate_kernel(uint8_t* store, float* sc
                                                        int kv_heads, int capacity, int block, int blocks,
                                                        const int64_t* move_from, const int64_t* move_to,
                                                        unsigned* err) {
-  constexpr int E = D / 32;
+  constexpr int kLanes = Lanes<D>::kLanes;
   pdl_wait();
   pdl_trigger();
   const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, rows = 32 / kLanes;
   if (item >= static_cast<long long>(planes) * batch * kv_heads) return;
   const int row = static_cast<int>(item / kv_heads % batch);
   const long long source = move_from[row], target = move_to[row];
@@ -239,31 +374,46 @@ __global__ void __launch_bounds__(128) relocate_kernel(uint8_t* store, float* sc
     if (lane == 0) raise_error(err, kErrBadShape);
     return;
   }
-  uint8_t* codes = store + static_cast<size_t>(item) * capacity * D + lane * E;
+  uint8_t* codes = store + static_cast<size_t>(item) * capacity * D + lane % kLanes * 4;
   float* s = scales + static_cast<size_t>(item) * blocks;
   const long long to_block = target / block, low = to_block * block;
-  float x[E];
-  load_codes<E>(codes + source * D, x);
-  const float from_scale = s[source / block], before = s[to_block];
   if (source / block == to_block) {  // one scale: the codes move as they are
-    store_codes<E>(codes + target * D, x, 1.f);
+    if (sub < 2)
+      *reinterpret_cast<uint32_t*>(codes + target * D + sub * (D / 2)) =
+          *reinterpret_cast<const uint32_t*>(codes + source * D + sub * (D / 2));
     return;
   }
+  float x[kE];
+  load_codes8<D>(codes + source * D, x);
+  const float from_scale = s[source / block], before = s[to_block];
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] *= from_scale;
-  const float wanted = least_scale(warp_max(finite_max<E>(x, 0.f)));
+  for (int e = 0; e < kE; ++e) x[e] *= from_scale;
+  const float wanted = least_scale(warp_max(finite_max(x, 0.f)));
   const bool joins = target > low;
   const float after = joins ? fmaxf(wanted, before) : wanted;
   const float inverse = 1.f / after;
   if (joins && after > before)
-    for (long long slot = low; slot < target; ++slot) {
-      float old[E];
-      load_codes<E>(codes + slot * D, old);
-      store_codes<E>(codes + slot * D, old, before * inverse);
+    for (long long slot = low + sub; slot < target; slot += rows) {
+      float old[kE];
+      load_codes8<D>(codes + slot * D, old);
+      store_codes8<D, true>(codes + slot * D, old, before * inverse);
     }
-  store_codes<E>(codes + target * D, x, inverse);
+  if (sub == 0) store_codes8<D, true>(codes + target * D, x, inverse);
   __syncwarp();
   if (lane == 0) s[to_block] = after;
+}
+
+constexpr long long kPromptRows = 1024;  // tokens from which Q heads and blocks take a launch each
+
+template <int D, bool kSplit>
+int launch_append(const AppendParams& p, long long rows, long long ctas, cudaStream_t s) {
+  const dim3 threads(kThreads);
+  if (rows < kPromptRows)
+    return launch_ex(append_kernel<D, kSplit, kBoth>, dim3(static_cast<unsigned>(ctas)), threads, 0, s, 1, p);
+  const int st = launch_ex(append_kernel<D, kSplit, kQueries>, dim3(p.query_ctas), threads, 0, s, 1, p);
+  if (st != FB_OK) return st;
+  return launch_ex(append_kernel<D, kSplit, kBlocks>, dim3(static_cast<unsigned>(ctas - p.query_ctas)), threads, 0, s, 1,
+                   p);
 }
 
 }  // namespace q8
@@ -284,6 +434,10 @@ extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, 
     return FB_ERR_ARG;
   if (mode < 0 || mode > 2 || (table && mode == 1) || (phases && !table)) return FB_ERR_ARG;
   if ((head_dim != 64 && head_dim != 128) || !q8::valid_block(block) || tokens > capacity) return FB_ERR_SHAPE;
+  // vector loads of the inputs and stores of the queries
+  for (const void* q : {packed, q_weight, k_weight, cos, sin, static_cast<const void*>(query),
+                        static_cast<const void*>(cache->keys), static_cast<const void*>(cache->values)})
+    if (reinterpret_cast<uintptr_t>(q) & 15u) return FB_ERR_ARG;
   q8::AppendParams p;
   p.packed = packed;
   p.splits = packed_splits;
@@ -306,21 +460,26 @@ extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, 
   p.kv_heads = kv_heads;
   p.capacity = capacity;
   p.block = block;
+  p.block_shift = block == 16 ? 4 : block == 32 ? 5 : 6;
   p.blocks = (capacity + block - 1) / block;
   p.mode = mode;
   p.table = table ? 1 : 0;
   p.err = error_word();
   // a prompt starts on a block; elsewhere the first token can be a block's last slot
   p.touched = mode == 1 ? (tokens + block - 1) / block : (tokens + block - 2) / block + 1;
-  const long long heads = static_cast<long long>(batch) * tokens * q_heads;
-  const long long query_ctas = (heads + q8::kWarps - 1) / q8::kWarps;
+  // a prompt's warps take eight heads of a token (four loads in flight at D = 128), a few rows' the least
+  // that fills a load, so that more warps share them
+  const long long rows = static_cast<long long>(batch) * tokens;
+  p.query_heads = rows >= q8::kPromptRows ? 8 : 32 * q8::kE / head_dim;
+  p.runs = (q_heads + p.query_heads - 1) / p.query_heads;
+  const long long query_ctas = (rows * p.runs + q8::kWarps - 1) / q8::kWarps;
   const long long ctas = query_ctas + 2ll * batch * kv_heads * p.touched;
-  if (ctas >= (1ll << 31) || static_cast<long long>(batch) * tokens >= (1ll << 31)) return FB_ERR_SHAPE;
+  if (ctas >= (1ll << 31) || rows * p.runs >= (1ll << 31)) return FB_ERR_SHAPE;
   p.query_ctas = static_cast<int>(query_ctas);
-  const dim3 grid(static_cast<unsigned>(ctas)), threads(q8::kThreads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_ex(q8::append_kernel<128>, grid, threads, 0, s, 1, p);
-  return launch_ex(q8::append_kernel<64>, grid, threads, 0, s, 1, p);
+  if (head_dim == 128)
+    return packed_splits ? q8::launch_append<128, true>(p, rows, ctas, s) : q8::launch_append<128, false>(p, rows, ctas, s);
+  return packed_splits ? q8::launch_append<64, true>(p, rows, ctas, s) : q8::launch_append<64, false>(p, rows, ctas, s);
 }
 
 extern "C" int fb_spec_relocate_q8(void* store, float* scales, int planes, int batch, int kv_heads, int capacity,

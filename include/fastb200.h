@@ -176,7 +176,7 @@ int fb_qk_norm_rope_append(const void* packed, int packed_splits, const void* q_
  * negative holds no sequence: nothing is appended to it and its attention output is zeros.
  *
  * fb_qk_norm_rope_append_q8: fb_qk_norm_rope_append for this cache: the same packed input,
- *   modes, phases and query output, but norm and RoPE stay in fp32 up to the one rounding (Q to
+ *   modes, phases and query output (all 16-byte aligned), but norm and RoPE stay in fp32 up to the one rounding (Q to
  *   bf16, K and V to e4m3, to nearest even). A block's scale is the least power of two s (at least 2^-100) such
  *   that the largest finite magnitude of its slots is <= 448 s; values that are not finite become
  *   the NaN code. A token in a block's first slot sets the scale anew; one that joins earlier slots
