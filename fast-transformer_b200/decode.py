@@ -33,10 +33,12 @@ from kernels import _native
 from kernels.argmax import argmax, fused_argmax
 from kernels.prefill import prefill_attention
 from kernels.decode_attention import attend as attend_decode
+from kernels.decode_attention import decode_attention_q8
 from kernels import linear as klinear
 from kernels.linear import linear, swiglu_linear
+from kernels.quant import CODE, QuantCache, Weight4
 from kernels.merged import Split
-from kernels.qk_rope import qk_rope_cache
+from kernels.qk_rope import qk_rope_cache, qk_rope_cache_q8
 from kernels.rmsnorm import add_rms_norm, embed_rms_norm
 from kernels.swiglu import swiglu
 from kernels._native import check, lib, ptr, stream
@@ -57,6 +59,29 @@ class KVCache:
         """K+V bytes of all layers for ``length`` valid slots per row."""
         _, layers, batch, kv_heads, _, dim = self.store.shape
         return 2 * layers * batch * kv_heads * length * dim * 2
+
+
+class QuantKVCache:
+    """The 8-bit form of ``KVCache``: e4m3 codes [2, layers, batch, kv_heads, capacity, head_dim] in one
+    allocation, fp32 scales per block of slots in another (no counterpart in the reference).
+    ``layers[i]`` is layer i's ``QuantCache``; ``kernels.spec.relocate_q8`` takes store and scales."""
+
+    def __init__(self, layers, batch, kv_heads, capacity, head_dim, device, block=64):
+        shape = (2, layers, batch, kv_heads, capacity, head_dim)
+        self.block = block
+        self.store = torch.zeros(shape, dtype=torch.uint8, device=device).view(CODE)
+        self.scales = torch.zeros((*shape[:4], -(-capacity // block)), dtype=torch.float32, device=device)
+        self.layers = [QuantCache(self.store[0, i], self.store[1, i], self.scales[0, i], self.scales[1, i], block)
+                       for i in range(layers)]
+
+    def row(self, layer, row):
+        """One row of one layer, as a cache of its own."""
+        return QuantCache(*(t[i, layer, row:row + 1] for t in (self.store, self.scales) for i in range(2)), self.block)
+
+    def nbytes_valid(self, length):
+        """K+V bytes of all layers (codes and scales) for ``length`` valid slots per row."""
+        _, layers, batch, kv_heads, _, dim = self.store.shape
+        return 2 * layers * batch * kv_heads * (length * dim + -(-length // self.block) * 4)
 
 
 def rope_tables(cfg, length, device):
@@ -198,9 +223,10 @@ def _allreduce_add_norm(x, weight, comm, peers, use, epoch, residual, gain, eps,
     width = residual.shape[-1]
     out = torch.empty_like(residual)
     summed = torch.empty_like(residual)
-    if splits is None:
+    if splits is None and not isinstance(weight, Weight4):
         splits = klinear.splits_for(rows, n, k, x.device)
     partials = klinear.project(flat, weight, klinear.SPLITS_OUT, splits)
+    splits = partials.shape[0]
     if peers.form == "push":
         check(lib.fb_allreduce_push(ptr(partials), splits, rows, n, comm.size, comm.rank, use, peers.recv_ptrs,
                                     ptr(epoch), stream()), "fb_allreduce_push")
@@ -216,23 +242,40 @@ def _allreduce_add_norm(x, weight, comm, peers, use, epoch, residual, gain, eps,
     return out, summed
 
 
+def _dense(weight):
+    """A projection's weights as a BF16 tensor, for the prompt's library products."""
+    return weight.dequantized() if isinstance(weight, Weight4) else weight
+
+
 class DecodeState:
     """KV cache, RoPE tables, device-side position and token ids, and the captured decode step.
+    ``kv_cache="q8"`` keeps the cache in 8 bits with a scale per head and ``kv_block`` slots
+    (``QuantKVCache``); the weights may be 4-bit (``qwen3.quantize_weights``).
 
     ``prefill(prompt)`` fills cache slots [0, T) and leaves the first greedy token in
     ``token_ids``; each ``step()`` replays the graph: one greedy token per row, written to
     ``token_ids``, KV appended at ``position``, ``position += 1``.
     """
 
-    def __init__(self, weights, batch, prompt_length, max_new_tokens, comm=None, device="cuda"):
+    def __init__(self, weights, batch, prompt_length, max_new_tokens, comm=None, device="cuda", kv_cache="bf16",
+                 kv_block=64):
+        if kv_cache not in ("bf16", "q8"):
+            raise ValueError(f"unknown KV cache form {kv_cache!r}")
         self.w = weights
+        self.quantised = kv_cache == "q8"
         self.cfg = weights.cfg
         self.comm = comm or Communicator()
         self.device = torch.device(device)
         self.batch, self.prompt_length = batch, prompt_length
         self.capacity = prompt_length + max_new_tokens
         cfg = self.cfg
-        self.cache = KVCache(cfg.num_hidden_layers, batch, weights.kv_heads, self.capacity, cfg.head_dim, self.device)
+        shape = (cfg.num_hidden_layers, batch, weights.kv_heads, self.capacity, cfg.head_dim, self.device)
+        if self.quantised:
+            self.cache = QuantKVCache(*shape, block=kv_block)
+            self.norms = [(_Norm(layer.q_norm, cfg.rms_norm_eps), _Norm(layer.k_norm, cfg.rms_norm_eps))
+                          for layer in weights.layers]
+        else:
+            self.cache = KVCache(*shape)
         self.cos, self.sin = rope_tables(cfg, self.capacity, self.device)
         self.position = torch.full((1,), prompt_length, dtype=torch.int64, device=self.device)
         self.token_ids = torch.zeros((batch, 1), dtype=torch.int64, device=self.device)
@@ -254,8 +297,13 @@ class DecodeState:
         attention (fb_decode_attention) for one layer. Fusing the norm/RoPE/append into the
         attention kernel's prologue measured slower on B200 (one TP8 rank's shard alone 2000
         against 1954 us per step): every CTA of a pair's cluster summed the qkv split partials
-        of its query heads on the attention's critical path."""
+        of its query heads on the attention's critical path. The 8-bit cache takes the same two
+        calls in its form (fb_qk_norm_rope_append_q8, fb_attention_q8)."""
         cache, w = self.cache, self.w
+        if self.quantised:
+            query = qk_rope_cache_q8(linear(normalized, layer.qkv, split_ok=True), *self.norms[index], self.cos, self.sin,
+                                     self.position, cache.layers[index], w.q_heads, table=True)
+            return decode_attention_q8(query, cache.layers[index], self.position, self.scale)
         keys, values = cache.keys[index], cache.values[index]
         query = _qkv_rope_decode(normalized, layer, self.cfg.rms_norm_eps, self.cos, self.sin, self.position, keys,
                                  values, w.q_heads)
@@ -270,7 +318,7 @@ class DecodeState:
         (one K split, the fused kernel's arithmetic) into ``self.logits`` and reduced by
         argmax instead - the same ids.
         """
-        w, cfg, cache, comm, peers = self.w, self.cfg, self.cache, self.comm, self.peers
+        w, cfg, comm, peers = self.w, self.cfg, self.comm, self.peers
         eps = cfg.rms_norm_eps
         layers = w.layers
         normalized, residual = embed_rms_norm(self.token_ids, w.embed, layers[0].ln1, eps)
@@ -360,6 +408,8 @@ class DecodeState:
         cos, sin = self.cos[:length][None].contiguous(), self.sin[:length][None].contiguous()
         last = torch.empty((batch, 1, cfg.hidden_size), dtype=BF16, device=self.device)
         last_residual = torch.empty_like(last)
+        scratch = [torch.empty((1, w.kv_heads, length, cfg.head_dim), dtype=BF16, device=self.device)
+                   for _ in range(2)] if self.quantised else None
         for row in range(batch):
             ids = prompt[row:row + 1]
             normalized, residual = embed_rms_norm(ids, w.embed, w.layers[0].ln1, eps)
@@ -367,18 +417,23 @@ class DecodeState:
             for index, layer in enumerate(w.layers):
                 if index > 0:
                     normalized, residual = add_rms_norm(hidden, residual, layer.ln1, eps)
-                keys = self.cache.keys[index][row:row + 1]
-                values = self.cache.values[index][row:row + 1]
-                packed = F.linear(normalized, layer.qkv)
-                query = qk_rope_cache(packed, _Norm(layer.q_norm, eps), _Norm(layer.k_norm, eps), cos, sin,
-                                      positions, keys, values, w.q_heads, prefill=True)
+                packed = F.linear(normalized, _dense(layer.qkv))
+                norms = _Norm(layer.q_norm, eps), _Norm(layer.k_norm, eps)
+                if self.quantised:
+                    # the prompt attends to its exact keys and values; later steps read their codes
+                    keys, values = scratch
+                    qk_rope_cache_q8(packed, *norms, cos, sin, positions, self.cache.row(index, row), w.q_heads,
+                                     prefill=True)
+                else:
+                    keys, values = self.cache.keys[index][row:row + 1], self.cache.values[index][row:row + 1]
+                query = qk_rope_cache(packed, *norms, cos, sin, positions, keys, values, w.q_heads, prefill=True)
                 attention = prefill_attention(query, keys[:, :, :length], values[:, :, :length], self.scale)
                 attention = attention.reshape(1, length, -1)
-                out = comm.all_reduce(F.linear(attention, layer.o))
+                out = comm.all_reduce(F.linear(attention, _dense(layer.o)))
                 normalized, residual = add_rms_norm(out, residual, layer.ln2, eps)
-                gate, up = qwen3.split_gate_up(layer.gate_up)
+                gate, up = qwen3.split_gate_up(_dense(layer.gate_up))
                 hidden = comm.all_reduce(F.linear(swiglu(torch.cat((F.linear(normalized, gate),
-                                                                      F.linear(normalized, up)), -1)), layer.down))
+                                                                      F.linear(normalized, up)), -1)), _dense(layer.down)))
             last[row] = hidden[0, -1:]
             last_residual[row] = residual[0, -1:]
         normalized, _ = add_rms_norm(last, last_residual, w.final_norm, eps)

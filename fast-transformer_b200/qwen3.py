@@ -12,7 +12,7 @@ gate/up, and the matching input columns of o_proj and down_proj; embeddings, nor
 """
 
 import hashlib
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
@@ -60,6 +60,7 @@ class Layer:
     o: torch.Tensor         # [H, q_local * D]
     gate_up: torch.Tensor   # [2 I_local, H]: 64-row gate/up blocks interleaved
     down: torch.Tensor      # [H, I_local]
+    # (the four projections may be kernels.quant.Weight4: quantize_weights)
 
 
 class Weights:
@@ -88,10 +89,20 @@ class Weights:
     def nbytes_per_step(self, vocab_parallel=True):
         """Weight bytes one decode step reads on this rank: every projection once and the LM
         head rows this rank projects (its vocabulary slice, or all of it)."""
-        per_layer = sum(t.numel() for t in (self.layers[0].qkv, self.layers[0].o, self.layers[0].gate_up,
-                                              self.layers[0].down)) * 2
+        per_layer = sum(t.nbytes for t in (self.layers[0].qkv, self.layers[0].o, self.layers[0].gate_up,
+                                             self.layers[0].down))
         head = self.lm_head_local if vocab_parallel else self.lm_head
         return per_layer * len(self.layers) + head.numel() * 2
+
+
+def quantize_weights(weights, group=128):
+    """The same model with its four projections per layer in 4 bits, one scale per row and ``group``
+    input columns (embeddings, norms and the LM head stay bf16). Needs the weights on the GPU."""
+    from kernels.quant import quantize_weight4
+    layers = [replace(layer, **{name: quantize_weight4(getattr(layer, name), group)
+                                for name in ("qkv", "o", "gate_up", "down")}) for layer in weights.layers]
+    return Weights(weights.cfg, layers, weights.embed, weights.final_norm, weights.lm_head, weights.tp_rank,
+                   weights.tp_size)
 
 
 BLOCK = 64
@@ -182,6 +193,8 @@ def to_state_dict(weights, device="cpu"):
     """HF-named tensors of an unsharded (TP 1) ``Weights``: the inverse of ``from_state_dict``."""
     if weights.tp_size != 1:
         raise ValueError("to_state_dict needs the whole model (tp_size 1)")
+    if not torch.is_tensor(weights.layers[0].qkv):
+        raise ValueError("to_state_dict needs bf16 projections (these are quantised)")
     cfg = weights.cfg
     d, hq, hkv, inter = cfg.head_dim, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.intermediate_size
     out = {"model.embed_tokens.weight": weights.embed.to(device), "model.norm.weight": weights.final_norm.to(device)}

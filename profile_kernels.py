@@ -162,9 +162,15 @@ def step(args):
     # --tp-size N: one rank's shard shapes (rank 0 of N), run alone, for per-kernel times at TP N
     # (the all-reduce consumers then run as the single-rank add+norm)
     weights = qwen3.random_init(cfg, "cuda", seed=0, tp_rank=0, tp_size=args.tp_size)
-    state = fdecode.DecodeState(weights, args.batch, args.length, 8)
+    if args.weight_group:
+        weights = qwen3.quantize_weights(weights, args.weight_group)
+    state = fdecode.DecodeState(weights, args.batch, args.length, 8, kv_cache=args.kv_cache)
     # decode cost does not depend on cache contents: random K/V instead of a prefill
-    state.cache.store.normal_()
+    if args.kv_cache == "q8":
+        state.cache.store.view(torch.uint8).random_(0, 0x70)
+        state.cache.scales.fill_(2.0 ** -7)
+    else:
+        state.cache.store.normal_()
     state.position.fill_(args.length)
     for _ in range(2):
         state.decode()
@@ -185,8 +191,8 @@ def step(args):
         end.record()
         end.synchronize()
         ms = start.elapsed_time(end) / 20
-        print(f"step {args.preset} TP-shard 1/{args.tp_size} B={args.batch} L={args.length}: "
-              f"{ms * 1e3:.1f} us per captured step ({args.batch / ms * 1e3:.0f} tok/s for this shard alone)")
+        print(f"step {args.preset} {args.kv_cache} cache, {'4-bit' if args.weight_group else 'bf16'} weights, "
+              f"TP-shard 1/{args.tp_size} B={args.batch} L={args.length}: {ms * 1e3:.1f} us per captured step ({args.batch / ms * 1e3:.0f} tok/s for this shard alone)")
         state.release()
         return
     torch.cuda.nvtx.range_push("profiled")
@@ -211,6 +217,8 @@ def main():
     parser.add_argument("--splits", type=int, default=0, help="linear: K splits (0: the library's choice)")
     parser.add_argument("--preset", default="qwen3-8b")
     parser.add_argument("--tp-size", type=int, default=1)
+    parser.add_argument("--kv-cache", default="bf16", choices=("bf16", "q8"), help="step: form of the KV cache")
+    parser.add_argument("--weight-group", type=int, default=0, help="step: 4-bit projections of this group (0: bf16)")
     parser.add_argument("--timed", action="store_true", help="step: time the captured step instead of profiling")
     parser.add_argument("--copies", type=int, default=2)
     parser.add_argument("--shapes", default="", help="attention: cluster-form shapes to sweep, e.g. 8x2,8x3,16x2")
