@@ -66,7 +66,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t kIdescS = tc::idesc_bf16(kTile, kTile, false, false);
   constexpr uint32_t kIdescO = tc::idesc_bf16(kTile, D, false, true);
   pdl_wait();
-  pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = base + S::kQOff;
@@ -116,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  pdl_trigger();  // only now: a dependent kernel's CTAs may take tensor memory of their own and wait for this one
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + kTmemO;
 
