@@ -13,8 +13,9 @@
 // Unpacking is exact: a nibble q = code + 8 in the low mantissa bits of 128.0 is the bf16 number
 // 128 + q; subtracting 136 leaves the code. W itself is never rounded, x stays bf16.
 //
-// Work: a cluster of `splits` CTAs owns `per` consecutive 128-row tiles and cuts their 128-column blocks
-// into equal contiguous ranges, one per CTA (per 2 and splits 3 turn 192 tiles into 288 even CTAs). The
+// Work: a cluster of `splits` CTAs owns a 128-row tile and cuts its 128-column blocks into equal
+// contiguous ranges, one per CTA. (Clusters of several tiles, for evener waves, gained 9% at 24576 x 4096
+// and lost 15% at small sizes.) The
 // packed layout keeps a block's codes and scales together, so a block is one bulk copy (8 KB and
 // 256 bytes a group) and two boxes of x. Warp roles: four unpacking warps, a producer lane, an MMA
 // lane; A is double-buffered and block b is unpacked while block b - 1 multiplies. The CTAs' totals
@@ -22,6 +23,9 @@
 // one launch, no workspace, the same bits every time, and the result leaves finished (bf16, fp32
 // or SwiGLU).
 #include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "tcgen05.cuh"
 
@@ -63,7 +67,6 @@ struct Params {
   const uint8_t* packed;
   void* out;
   int m, n, epilogue;
-  int per;  // tiles of a cluster
   Layout layout;
   unsigned* err;
 };
@@ -126,7 +129,6 @@ __device__ __forceinline__ uint32_t codes_bf16x2(uint32_t w, const Magic& k) {
 template <int M_, int SEGS_>
 struct Config {
   static constexpr int M = M_, SEGS = SEGS_;
-  static constexpr int TILES = 1;  // of a cluster at most
   // A block is unpacked and multiplied in one part, or in two where its groups' D would not fit.
   static constexpr int PARTS = SEGS * M > 192 ? 2 : 1, kPart = kBlock / PARTS, GROUPS = SEGS / PARTS;
   // tensor memory: per set an A buffer of kPart / 2 columns and a D of M columns a group. Two CTAs share
@@ -139,8 +141,8 @@ struct Config {
   static constexpr int kX = 2 * kBoxBytes;
   static constexpr int kW = 9 * 1024;  // codes and at most four groups' scales
   static constexpr int kStage = kX + kW;
-  // totals received as an owner: [tile][rank][set][column][local row], at most 2 ceil(64 / S) S <= 142 rows a tile
-  static constexpr int kRecv = TILES * kSets * 142 * M * 4;
+  // totals received as an owner: [rank][set][column][local row], at most 2 ceil(64 / S) S <= 142 rows
+  static constexpr int kRecv = kSets * 142 * M * 4;
   static constexpr int kFree = (228 * 1024) / kCtas - 1024 - 1024 - kRecv - 256;
   static constexpr int NS = kFree / kStage > 8 ? 8 : kFree / kStage;
   static constexpr int kTotal = 1024 + NS * kStage + kRecv + 256;
@@ -164,17 +166,11 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;
-  const int blocks = p.layout.blocks();  // of a tile
-  const int tile0 = blockIdx.y * p.per, tiles = min(p.per, p.layout.tiles - tile0);
-  const int all = tiles * blocks;  // of the cluster; this CTA: [b0, b0 + count)
-  const int sharers = min(splits, all);  // CTAs that have blocks
-  auto first_block = [&](int r) { return static_cast<int>(static_cast<long long>(all) * min(r, sharers) / sharers); };
-  const int b0 = first_block(rank), count = first_block(rank + 1) - b0;
+  const int tile = blockIdx.y, blocks = p.layout.blocks();  // of a tile; this CTA: [b0, b0 + count)
+  const int b0 = blocks * rank / splits, count = blocks * (rank + 1) / splits - b0;
   const int parts = count * PARTS;  // part i: stage i / PARTS, columns_of(i) columns (none at a short block's end)
-  static_assert(C::TILES <= 2, "a block index passes the tile's end at most once");
-  auto block_of = [&](int j) { return b0 + j < blocks ? b0 + j : b0 + j - blocks; };
   auto columns_of = [&](int i) {
-    return max(0, min(C::kPart, p.layout.columns(block_of(i / PARTS)) - i % PARTS * C::kPart));
+    return max(0, min(C::kPart, p.layout.columns(b0 + i / PARTS) - i % PARTS * C::kPart));
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -213,8 +209,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
   if (warp == kProducerWarp) {
     const uint64_t policy = l2_evict_first_policy();
     auto weights = [&](int i) {
-      const int s = i % NS, block = block_of(i), bytes = p.layout.bytes(block);
-      const uint8_t* src = p.packed + p.layout.at(tile0 + (b0 + i >= blocks), block);
+      const int s = i % NS, bytes = p.layout.bytes(b0 + i);
+      const uint8_t* src = p.packed + p.layout.at(tile, b0 + i);
       if (elect_one()) {
         mbar_arrive_expect_tx(&full[s], bytes + C::kX);
         bulk_load(ring + s * C::kStage + C::kX, src, bytes, &full[s], policy);
@@ -222,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
       __syncwarp();
     };
     auto inputs = [&](int i) {
-      const int s = i % NS, column = block_of(i) * kBlock;
+      const int s = i % NS, column = (b0 + i) * kBlock;
       uint8_t* at = ring + s * C::kStage;
       if (elect_one()) {
         tma_load_2d(at, &xmap, &full[s], column, 0);
@@ -291,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 #pragma unroll
       for (int r = 0; r < kRuns; ++r)  // runs and groups past the last block's columns read what is not used
         codes[r] = *reinterpret_cast<const uint4*>(at + (part * kRuns + r) * kRunBytes + row * 16);
-      const uint8_t* scales = at + p.layout.columns(block_of(j)) / kRun * kRunBytes + row * 2;
+      const uint8_t* scales = at + p.layout.columns(b0 + j) / kRun * kRunBytes + row * 2;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
         scale[g] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(scales + (part * GROUPS + g) * kRows * 2));
@@ -302,56 +298,53 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     const int share = (64 + splits - 1) / splits;  // features (rows f and f + 64) of an owner
     const int f64 = row & 63, owner = f64 / share, local = (row >> 6) * share + f64 - owner * share;
     float total[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) total[m] = 0.f;
     bool ok = set >= parts || fetch(set);
-    int i = set;                     // this set's parts: set, set + kSets, ...
     if (splits > 1) cluster_wait();  // every CTA of the cluster runs
-    // the tiles that this CTA's range touches, each set's share of each pushed to the owners
-    for (int t = b0 >= blocks; ok && count > 0 && t * blocks < b0 + count; ++t) {
+    for (int i = set; ok && i < parts; i += kSets) {  // this set's parts
+      const int turn = i / kSets, groups = columns_of(i) >> p.layout.group_shift;
+      // A is free: the products of this set's last block were waited for below
 #pragma unroll
-      for (int m = 0; m < M; ++m) total[m] = 0.f;
-      const int end = min(parts, ((t + 1) * blocks - b0) * PARTS);
-      for (; ok && i < end; i += kSets) {
-        const int turn = i / kSets, groups = columns_of(i) >> p.layout.group_shift;
-        // A is free: the products of this set's last block were waited for below
+      for (int r = 0; r < kRuns; ++r) {
+        const uint32_t words[4] = {codes[r].x, codes[r].y, codes[r].z, codes[r].w};
+        uint32_t a[16];
 #pragma unroll
-        for (int r = 0; r < kRuns; ++r) {
-          const uint32_t words[4] = {codes[r].x, codes[r].y, codes[r].z, codes[r].w};
-          uint32_t a[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            a[4 * j] = codes_bf16x2(words[j], magic);
-            a[4 * j + 1] = codes_bf16x2(words[j] >> 4, magic);
-            a[4 * j + 2] = codes_bf16x2(words[j] >> 8, magic);
-            a[4 * j + 3] = codes_bf16x2(words[j] >> 12, magic);
-          }
-          st16(a_lanes + r * 16, a);
+        for (int j = 0; j < 4; ++j) {
+          a[4 * j] = codes_bf16x2(words[j], magic);
+          a[4 * j + 1] = codes_bf16x2(words[j] >> 4, magic);
+          a[4 * j + 2] = codes_bf16x2(words[j] >> 8, magic);
+          a[4 * j + 3] = codes_bf16x2(words[j] >> 12, magic);
         }
-        wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[set]);
-        float f[GROUPS];
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) f[g] = scale[g];
-        ok = i + kSets >= parts || fetch(i + kSets);  // while the part multiplies
-        ok = ok && __all_sync(0xffffffffu, wait(&d_full[set], turn & 1, kErrTimeoutMma));
-        if (!ok) break;
-        tc::fence_after();
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          if (g >= groups) break;
-#pragma unroll
-          for (int c = 0; c < M; c += 16) {
-            float v[16];
-            tc::ld16(d_lanes + g * M + c, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) total[c + e] += v[e] * f[g];
-          }
-        }
-        tc::fence_before();  // the next a_full says that D was read
+        st16(a_lanes + r * 16, a);
       }
-      const uint32_t dst = map_shared(
-          smem_u32(recv + ((t * splits + rank) * kSets + set) * M * 2 * share + local), owner);
+      wait_st();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[set]);
+      float f[GROUPS];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) f[g] = scale[g];
+      ok = i + kSets >= parts || fetch(i + kSets);  // while the part multiplies
+      ok = ok && __all_sync(0xffffffffu, wait(&d_full[set], turn & 1, kErrTimeoutMma));
+      if (!ok) break;
+      tc::fence_after();
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        if (g >= groups) break;
+#pragma unroll
+        for (int c = 0; c < M; c += 16) {
+          float v[16];
+          tc::ld16(d_lanes + g * M + c, v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) total[c + e] += v[e] * f[g];
+        }
+      }
+      tc::fence_before();  // the next a_full says that D was read
+    }
+    if (ok) {
+      const uint32_t dst =
+          map_shared(smem_u32(recv + (rank * kSets + set) * M * 2 * share + local), owner);
 #pragma unroll
       for (int m = 0; m < M; ++m)
         if (m < p.m) st_cluster_f32(dst + m * 2 * share * 4, total[m]);
@@ -371,28 +364,22 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     const int per = kUnpackWarps * 32 / wide;  // columns that the threads cover at once
     const int at = threadIdx.x % wide, m0 = threadIdx.x / wide;
     const int hi = at >= mine ? 1 : 0, f = at - hi * mine;
-    for (int t = 0; t < tiles && m0 < per; ++t) {
-      const int tile = tile0 + t, n = tile * kRows + hi * 64 + rank * share + f;
-      if (n >= p.n) break;
-      int low = 0, high = sharers - 1;  // the ranks whose ranges meet the tile's blocks
-      while (first_block(low + 1) <= t * blocks) ++low;
-      while (first_block(high) >= (t + 1) * blocks) --high;
-      auto sum = [&](int m, int half) {
-        const float* src = recv + ((t * splits + low) * kSets * M + m) * 2 * share + half * share + f;
-        float v = src[0];
-        for (int q = 1; q < (high - low + 1) * kSets; ++q) v += src[q * M * 2 * share];
-        return v;
-      };
-      for (int m = m0; m < p.m; m += per) {
-        if (p.epilogue == kSwiGLU) {
-          const float gate = bf16_round(sum(m, 0)), up = bf16_round(sum(m, 1));
-          static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * (p.n / 2) + tile * 64 + rank * share + f] =
-              __float2bfloat16_rn(bf16_round(gate / (1.0f + expf(-gate))) * up);
-        } else if (p.epilogue == kFp32) {
-          static_cast<float*>(p.out)[static_cast<size_t>(m) * p.n + n] = sum(m, hi);
-        } else {
-          static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * p.n + n] = __float2bfloat16_rn(sum(m, hi));
-        }
+    const int n = tile * kRows + hi * 64 + rank * share + f;
+    auto sum = [&](int m, int half) {
+      const float* src = recv + m * 2 * share + half * share + f;
+      float v = src[0];
+      for (int q = 1; q < splits * kSets; ++q) v += src[q * M * 2 * share];
+      return v;
+    };
+    for (int m = m0; m0 < per && n < p.n && m < p.m; m += per) {
+      if (p.epilogue == kSwiGLU) {
+        const float gate = bf16_round(sum(m, 0)), up = bf16_round(sum(m, 1));
+        static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * (p.n / 2) + tile * 64 + rank * share + f] =
+            __float2bfloat16_rn(bf16_round(gate / (1.0f + expf(-gate))) * up);
+      } else if (p.epilogue == kFp32) {
+        static_cast<float*>(p.out)[static_cast<size_t>(m) * p.n + n] = sum(m, hi);
+      } else {
+        static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * p.n + n] = __float2bfloat16_rn(sum(m, hi));
       }
     }
   }
@@ -488,7 +475,7 @@ constexpr int kMaxDevices = 64;
 // Clusters of `splits` CTAs of a kernel that the device holds at once, kept per device.
 template <typename C>
 int resident_clusters(int splits) {
-  static int cache[kMaxDevices][kMaxSplits + 1] = {};  // count + 1; 0: not asked
+  static std::atomic<int> cache[kMaxDevices][kMaxSplits + 1];  // count + 1; 0: not asked
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < kMaxDevices && cache[dev][splits] != 0) return cache[dev][splits] - 1;
@@ -514,32 +501,32 @@ int resident_clusters(int splits) {
   return n;
 }
 
-// What a CTA costs beside its stream, in blocks.
+// What a CTA costs beside its stream, in blocks: 3 us at 0.35 us a block.
 constexpr int kFixed = 8;
 
-// K splits and tiles per cluster: the least waves x (blocks of a CTA + what it costs beside them). The
-// occupancy query counts one CTA per SM for kernels with tensor memory; kCtas share one.
+// K splits: the least waves x (blocks of a CTA + what it costs beside them). Clusters that the device holds:
+// the occupancy query counts one CTA per SM for kernels with tensor memory. Two share an SM where kCtas is 2,
+// so a cluster of S also fits wherever one of S / 2 does with a CTA to an SM. At M = 16 it takes 8 for
+// 4096 x 12288 (11.9 us; 6: 13.9, 4: 16.5, 1: 47.6) and 1 for 24576 x 4096 (22.5; 2: 21.8, 4: 26.5, 8: 44.0).
 template <typename C>
-int launch(const CUtensorMap& xm, Params p, cudaStream_t stream) {
-  const int blocks = p.layout.blocks();
+int launch(const CUtensorMap& xm, const Params& p, cudaStream_t stream) {
+  const int blocks = p.layout.blocks(), tiles = p.layout.tiles;
+  if (tiles > 65535) return FB_ERR_SHAPE;
   int best = 0;
   long long best_cost = 0;
-  for (int per = 1; per <= C::TILES && per <= p.layout.tiles; ++per)
-    for (int splits = 1; splits <= kMaxSplits && splits <= per * blocks; ++splits) {
-      const int slots = resident_clusters<C>(splits) * C::kCtas;
-      if (slots <= 0) continue;
-      const long long clusters = (p.layout.tiles + per - 1) / per, waves = (clusters + slots - 1) / slots;
-      const long long cost = waves * ((per * blocks + splits - 1) / splits + kFixed);
-      if (best == 0 || cost < best_cost) {
-        best = splits;
-        best_cost = cost;
-        p.per = per;
-      }
+  for (int splits = 1; splits <= kMaxSplits && splits <= blocks; ++splits) {
+    int slots = resident_clusters<C>(splits) * C::kCtas;
+    if (C::kCtas > 1) slots = std::max(slots, resident_clusters<C>((splits + 1) / 2));
+    if (slots <= 0) continue;
+    const long long waves = (tiles + slots - 1) / slots;
+    const long long cost = waves * ((blocks + splits - 1) / splits + kFixed);
+    if (best == 0 || cost < best_cost) {
+      best = splits;
+      best_cost = cost;
     }
+  }
   if (best == 0) return FB_ERR_LAUNCH;
-  const int clusters = (p.layout.tiles + p.per - 1) / p.per;
-  if (clusters > 65535) return FB_ERR_SHAPE;
-  return launch_ex(linear_w4_kernel<C>, dim3(best, clusters), dim3(kThreads), C::kTotal, stream, best, xm, p);
+  return launch_ex(linear_w4_kernel<C>, dim3(best, tiles), dim3(kThreads), C::kTotal, stream, best, xm, p);
 }
 
 template <int M>
