@@ -16,10 +16,15 @@
 // Bound by the bytes of codes. Members = the T * G query heads that share a KV head, in groups of
 // 8 NG columns; a unit = (row, KV head, member group); its tiles are 128 slots of K and V. A CTA is
 // a producer warp (one lane issues a TMA load per K and V tile, 16 lanes copy the tile's scales
-// with cp.async; both complete on the stage's mbarrier) and four consumer warps of two 16-slot
-// slices each: S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a score passes it by more
-// than 8, one vote), O^T += V^T P^T. Two CTAs share an SM: one streams while the other starts or
-// ends.
+// with cp.async; both complete on the stage's mbarrier) and consumer warps; two CTAs share an SM: one
+// streams while the other starts or ends. S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a
+// score passes it by more than 8, one vote), O^T += V^T P^T.
+//  * One column group: four consumers of two 16-slot slices each, whole in registers; a warp needs no
+//    other until the end.
+//  * More: the conversions and products of a tile, not its bytes, fill its time, and O^T of every warp
+//    would not fit the registers. Eight consumers: each scores its slice, P^T goes to shared memory, and
+//    each multiplies all of it by its 16 dims of V. One barrier a tile (the vote), O held once.
+// Work is cut in one of two ways:
 //  * Few units: a cluster of C CTAs per unit (interleaved tiles), merged by pushing each
 //    partial to its output's owner through distributed shared memory: one launch, no workspace.
 //  * Many units: a persistent grid cuts the tiles of all units into equal contiguous slices, so
@@ -33,10 +38,12 @@
 namespace fb {
 namespace attn8 {
 
-constexpr int kWarps = 4;  // consumers
-constexpr int kSlices = 2 * kWarps;  // of 16 slots: warp w takes slices 2 w and 2 w + 1
+constexpr int kSlices = 8;  // of 16 slots
 constexpr int kTile = 16 * kSlices;
-constexpr int kThreads = (kWarps + 1) * 32;
+template <int NG>
+constexpr int kConsumers = NG == 1 ? 4 : kSlices;  // warps
+template <int NG>
+constexpr int kThreads = (kConsumers<NG> + 1) * 32;
 constexpr int kMaxBatch = 1024;
 constexpr int kScales = 2 * kSlices;  // per stage: K and V scale of each 16-slot slice
 constexpr int kMaxCluster = 16;      // above 8: the non-portable cluster size attribute
@@ -112,27 +119,31 @@ template <int D, int NG>
 struct Smem {
   static constexpr int kTileBytes = kTile * D;
   // two CTAs per SM (asserted below): what the buffers of more column groups leave
-  static constexpr int kStages = D == 128 ? (NG == 1 ? 3 : 2) : 5;
+  static constexpr int kStages = D == 128 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 5 : 4);
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kScaleBytes = kStages * kScales * 4;
   static constexpr int kQueryPitch = D * 2 + 32;  // f16 query rows, padded against bank conflicts
   static constexpr int kQuery = NG == 1 ? 0 : NG * 8 * kQueryPitch;
-  static constexpr int kRedO = kWarps * D / 2 * 8 * 4;       // half the dims of an 8-column group of every warp
-  static constexpr int kRedStats = kWarps * NG * 8 * 3 * 4;  // M, m, l
+  // P^T as B fragments, [slice][group][lane], of two tiles in turn
+  static constexpr int kWeights = NG == 1 ? 0 : 2 * kSlices * NG * 32 * 8;
+  // one group: half the dims of every warp; more: the O of warps that share dims with others
+  static constexpr int kRedO = NG == 1 ? 4 * D / 2 * 8 * 4 : kSlices * NG * 32 * 16 / 2 * (D == 64);
+  static constexpr int kRedStats = NG == 1 ? kConsumers<NG> * 8 * 3 * 4 : 0;  // M, m, l
   // persistent form: tile counts before each row; cluster form: O received as an owner
-  // ([rank][chunk], C * ceil(n / C) <= n + C - 1 values) and every rank's M, m, l
+  // ([rank][chunk], C * 2 ceil(n / 2C) < n + 2C values) and every rank's M, m, l
   static constexpr int kCum = ((kMaxBatch + 1) * 4 + 15) & ~15;
-  static constexpr int kRecvO = (NG * 8 * D + kMaxCluster) * 4;
+  static constexpr int kRecvO = (NG * 8 * D + 2 * kMaxCluster) * 4;
   static constexpr int kRecvStats = kMaxCluster * NG * 8 * 3 * 4;
   static constexpr int kShared = kCum > kRecvO + kRecvStats ? kCum : kRecvO + kRecvStats;
   static constexpr int kBars = 2 * kStages * 8;
-  static constexpr int kTotal = 1024 + kRing + kScaleBytes + kQuery + kRedO + kRedStats + kShared + kBars + 32;
+  static constexpr int kTotal = 1024 + kRing + kScaleBytes + kQuery + kWeights + kRedO + kRedStats + kShared + kBars + 32;
   static_assert(kTotal + 1024 <= 228 * 1024 / 2, "two CTAs per SM");
-  static_assert((kScaleBytes + kQuery + kRedO + kRedStats + kShared) % 16 == 0, "mbarrier alignment");
+  static_assert((kScaleBytes + kQuery + kWeights + kRedO + kRedStats + kShared) % 16 == 0, "mbarrier alignment");
 
   uint8_t* ring;
   float* scales;
   uint8_t* query;
+  uint8_t* weights;
   float* red_o;
   float* red_stats;
   int* cum;
@@ -146,7 +157,8 @@ struct Smem {
     ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     scales = reinterpret_cast<float*>(ring + kRing);
     query = ring + kRing + kScaleBytes;
-    red_o = reinterpret_cast<float*>(query + kQuery);
+    weights = query + kQuery;
+    red_o = reinterpret_cast<float*>(weights + kWeights);
     red_stats = red_o + kRedO / 4;
     cum = reinterpret_cast<int*>(red_stats + kRedStats / 4);
     recv_o = reinterpret_cast<float*>(cum);
@@ -157,25 +169,41 @@ struct Smem {
   }
 };
 
-// A consumer warp's state on one unit. At one column group the query's B fragments stay in
-// registers; with more they are read from shared memory for every tile (the accumulators need
-// the registers).
+// A consumer warp's state on one unit. One column group: its slices' share of O^T, and the query's B
+// fragments. More: 16 dims of the unit's O^T and pivots that all warps hold alike; queries are read
+// from shared memory for every tile.
 template <int D, int NG>
 struct State {
+  static constexpr int kDims = NG == 1 ? D / 16 : 1;
   uint32_t q[NG == 1 ? D / 16 : 1][2];
-  float o[NG][D / 16][4];
+  float o[NG][kDims][4];
   float m[NG][2], M[NG][2], l[NG][2];  // columns 2c, 2c + 1
   float qs[NG][2];                     // score multiplier of those columns: 2^e scale log2(e)
 };
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32) : "memory"); }
+template <int NG>
+__device__ __forceinline__ void consumers_sync() {
+  asm volatile("bar.sync 1, %0;" ::"r"(kConsumers<NG> * 32) : "memory");
+}
+// The same barrier; whether any consumer thread says so.
+template <int NG>
+__device__ __forceinline__ bool consumers_any(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(any)
+      : "r"(x ? 1u : 0u), "r"(kConsumers<NG> * 32)
+      : "memory");
+  return any != 0;
+}
 
 template <int D, int NG>
 __device__ __forceinline__ void clear(State<D, NG>& a) {
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) a.o[n][k][0] = a.o[n][k][1] = a.o[n][k][2] = a.o[n][k][3] = 0.f;
+    for (int k = 0; k < State<D, NG>::kDims; ++k) a.o[n][k][0] = a.o[n][k][1] = a.o[n][k][2] = a.o[n][k][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       a.m[n][e] = a.M[n][e] = -INFINITY;
@@ -192,12 +220,10 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
                                            int warp, int lane) {
   using S = Smem<D, NG>;
   const int g = lane >> 2, c = lane & 3;
-  if (NG > 1) consumers_sync();  // the last unit's queries have been read
-#pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    if (NG > 1 && n % kWarps != warp) continue;  // with shared queries each warp converts its groups
-    const int member = chunk * p.width + n * 8 + g;
-    const bool live = n * 8 + g < p.width && member < p.members;
+  if (NG > 1) consumers_sync<NG>();  // the last unit's queries and totals have been read
+  if (warp < NG || NG == 1) {         // shared queries: a warp converts a group
+    const int col = NG == 1 ? g : warp * 8 + g, member = chunk * p.width + col;
+    const bool live = col < p.width && member < p.members;
     const int t = live ? member / p.groups : 0;
     const int head = h * p.groups + (live ? member - t * p.groups : 0);
     const __nv_bfloat16* row = p.q + ((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D;
@@ -217,6 +243,7 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
     const int first = up / 2;
     const float f0 = __uint_as_float(static_cast<uint32_t>(127 + first) << 23);
     const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up - first) << 23);
+    uint8_t* mine = query + col * S::kQueryPitch;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const uint32_t b0 = pack_f16x2(bf16_lo(w[k].x) * f0 * f1, bf16_hi(w[k].x) * f0 * f1);
@@ -225,19 +252,20 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
         a.q[k][0] = b0;
         a.q[k][1] = b1;
       } else {
-        *reinterpret_cast<uint2*>(query + (n * 8 + g) * S::kQueryPitch + (k * 16 + 4 * c) * 2) = make_uint2(b0, b1);
+        *reinterpret_cast<uint2*>(mine + (k * 16 + 4 * c) * 2) = make_uint2(b0, b1);
       }
     }
-    const float mine = p.scale_log2 / f0 / f1;  // of column g; this thread's scores are 2c and 2c + 1
+    const float multiplier = p.scale_log2 / f0 / f1;  // of column g; this thread's scores are 2c and 2c + 1
     if constexpr (NG == 1) {
-      a.qs[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
-      a.qs[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+      a.qs[0][0] = __shfl_sync(0xffffffffu, multiplier, 8 * c);
+      a.qs[0][1] = __shfl_sync(0xffffffffu, multiplier, 8 * c + 4);
     } else if (c == 0) {
-      *reinterpret_cast<float*>(query + (n * 8 + g) * S::kQueryPitch + D * 2) = mine;
+      *reinterpret_cast<float*>(mine + D * 2) = multiplier;
+      *reinterpret_cast<int*>(mine + D * 2 + 4) = t;
     }
   }
   if constexpr (NG > 1) {
-    consumers_sync();
+    consumers_sync<NG>();
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -247,27 +275,31 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
   clear<D, NG>(a);
 }
 
-// O^T += V^T P^T for 16 slots (`row`: this lane's row of the tile, `half`: its 16-byte chunk's parity).
-// Each register of a transposed load holds two dims of two slots; one byte permute and two
-// conversions make the A fragments of dims 2g (rows 0-7 of the product) and 2g + 1 (rows 8-15).
-// pick0 / pick1 are the permutes of slots (2c, 2c + 1) and 8 later: kPick, or with selectors of 4
-// (a zero byte) for slots left out.
+// A register of a transposed load of V holds two dims of two slots; one byte permute and two conversions
+// make the A fragments of dims 2g (rows 0-7 of the product) and 2g + 1 (rows 8-15). r0 holds slots
+// (2c, 2c + 1) of 16, r1 those 8 later; pick0 / pick1 are their permutes: kPick, or with selectors of 4 (a
+// zero byte) for slots left out.
 constexpr uint32_t kPick = 0x3120u;
 
-template <int D, int NG>
-__device__ __forceinline__ void value_product(float (&o)[NG][D / 16][4], uint32_t tile, int row, int half,
-                                              uint32_t pick0, uint32_t pick1, const uint32_t (&pb)[NG][2]) {
+__device__ __forceinline__ void value_fragments(uint32_t (&f)[4], uint32_t r0, uint32_t r1, uint32_t pick0,
+                                                uint32_t pick1) {
+  q8::e4m3x4_to_f16x4(__byte_perm(r0, 0, pick0), f[0], f[1]);
+  q8::e4m3x4_to_f16x4(__byte_perm(r1, 0, pick1), f[2], f[3]);
+}
+
+// O^T += V^T P^T for 16 slots and every dim (`row`: this lane's row of the tile, `half`: its 16-byte
+// chunk's parity).
+template <int D>
+__device__ __forceinline__ void value_product(float (&o)[D / 16][4], uint32_t tile, int row, int half, uint32_t pick0,
+                                              uint32_t pick1, const uint32_t (&pb)[2]) {
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
-    uint32_t r[4];
+    uint32_t r[4], f[4];
     ldmatrix_x4_trans(tile + swizzled<D>(row, 2 * i + half), r[0], r[1], r[2], r[3]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t a0, a1, a2, a3;
-      q8::e4m3x4_to_f16x4(__byte_perm(r[2 * j], 0, pick0), a0, a1);
-      q8::e4m3x4_to_f16x4(__byte_perm(r[2 * j + 1], 0, pick1), a2, a3);
-#pragma unroll
-      for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * i + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      value_fragments(f, r[2 * j], r[2 * j + 1], pick0, pick1);
+      mma_f16(o[2 * i + j], f[0], f[1], f[2], f[3], pb[0], pb[1]);
     }
   }
 }
@@ -284,6 +316,9 @@ __device__ __forceinline__ bool sees(int slot, int len, int position, int t, int
   return slot <= position || (t < chain ? slot <= position + t : slot == position + t);
 }
 
+// Whether a byte of w is a NaN code (0x7f or 0xff): adding 1 reaches its top bit.
+__device__ __forceinline__ bool has_nan(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+
 // Whether rows [row0, row0 + 16) of a tile hold a NaN code.
 template <int D>
 __device__ __forceinline__ bool any_nan(uint32_t tile, int row0, int lane) {
@@ -291,8 +326,7 @@ __device__ __forceinline__ bool any_nan(uint32_t tile, int row0, int lane) {
   for (int i = lane; i < 16 * D / 4; i += 32) {
     uint32_t w;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(tile + row0 * D + i * 4) : "memory");
-    w &= 0x7f7f7f7fu;  // a byte of 0x7f: adding 1 reaches its top bit
-    found = found || ((w + 0x01010101u) & 0x80808080u) != 0;
+    found = found || has_nan(w);
   }
   return __any_sync(0xffffffffu, found);
 }
@@ -304,172 +338,321 @@ __device__ __forceinline__ float log2_scale(float x) {
   return y;
 }
 
-// This warp's two slices of the 128-slot tile that starts at slot `first`. `len`: slots of the row;
-// `position`: its first token's slot; scales: the tile's, K then V. Up to two column groups the
-// slices run side by side (two independent chains hide each other's latency), else in turn.
-template <int D, int NG>
-__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const uint8_t* query,
-                                            const float* scales, uint32_t kt, uint32_t vt, int first, int len,
-                                            int position, int chain, int chunk, int warp, int lane) {
-  constexpr int H = NG <= 2 ? 2 : 1;
+// One column group: this warp's slices 2 w and 2 w + 1 of the 128-slot tile that starts at slot
+// `first`, side by side (two independent chains hide each other's latency). `len`: slots of the row;
+// `position`: its first token's slot; scales: the tile's, K then V.
+template <int D>
+__device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, const Smem<D, 1>&, const float* scales,
+                                            uint32_t kt, uint32_t vt, int, bool, int first, int len, int position, int chain,
+                                            int chunk, int warp, int lane) {
+  constexpr int H = 2;
   const int g = lane >> 2, c = lane & 3, half = lane >> 4;
-#pragma unroll 1
-  for (int s0 = 0; s0 < 2; s0 += H) {
-    const int slice = first + (warp * 2 + s0) * 16;
-    if (slice >= len) return;
-    const int row = (warp * 2 + s0) * 16 + (lane & 15);
-    float s[H][NG][4], s2[H][NG][4];
+  const int slice = first + warp * 32;
+  if (slice >= len) return;
+  const int row = warp * 32 + (lane & 15);
+  float s[H][4], s2[H][4];
+#pragma unroll
+  for (int x = 0; x < H; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int x = 0; x < H; ++x) {
+      uint32_t r[4], k0[4], k1[4];
+      ldmatrix_x4(kt + swizzled<D>(row + 16 * x, 2 * i + half), r[0], r[1], r[2], r[3]);
+      q8::e4m3x4_to_f16x4(r[0], k0[0], k0[2]);
+      q8::e4m3x4_to_f16x4(r[1], k0[1], k0[3]);
+      q8::e4m3x4_to_f16x4(r[2], k1[0], k1[2]);
+      q8::e4m3x4_to_f16x4(r[3], k1[1], k1[3]);
+      // two chains of products: half the latency
+      mma_f16(s[x], k0[0], k0[1], k0[2], k0[3], a.q[2 * i][0], a.q[2 * i][1]);
+      mma_f16(s2[x], k1[0], k1[1], k1[2], k1[3], a.q[2 * i + 1][0], a.q[2 * i + 1][1]);
+    }
+  float lv[H];
+#pragma unroll
+  for (int x = 0; x < H; ++x) {
+    const bool live = slice + 16 * x < len;  // past the row a scale can be anything
+    const float ks = live ? scales[warp * 2 + x] : 1.f;
+    lv[x] = live ? log2_scale(scales[kSlices + warp * 2 + x]) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[x][e] = (s[x][e] + s2[x][e]) * (a.qs[0][e & 1] * ks);
+  }
+  // every member sees slots [0, position]; past them the chain rule decides per token
+  const bool tail = slice + 16 * H > (p.chain != nullptr ? position + 1 : len);
+  if (tail) {
 #pragma unroll
     for (int x = 0; x < H; ++x)
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][n][e] = s2[x][n][e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      uint2 b0[NG], b1[NG];
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        if constexpr (NG == 1) {
-          b0[n] = make_uint2(a.q[2 * i][0], a.q[2 * i][1]);
-          b1[n] = make_uint2(a.q[2 * i + 1][0], a.q[2 * i + 1][1]);
-        } else {
-          const uint8_t* src = query + (n * 8 + g) * Smem<D, NG>::kQueryPitch + (i * 32 + 4 * c) * 2;
-          b0[n] = *reinterpret_cast<const uint2*>(src);
-          b1[n] = *reinterpret_cast<const uint2*>(src + 32);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int slot = slice + 16 * x + g + (e >> 1) * 8;
+        const int t = p.chain != nullptr ? (chunk * p.width + 2 * c + (e & 1)) / p.groups : 0;
+        if (!sees(slot, len, position, t, chain)) s[x][e] = -INFINITY;
       }
+  }
+  bool moves = false;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int x = 0; x < H; ++x)
+      moves = moves || fmaxf(s[x][e], s[x][e + 2]) > fminf(a.m[0][e], a.M[0][e] - lv[x]) + kSlack;
+  if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float m = a.m[0][e], M = a.M[0][e];
 #pragma unroll
       for (int x = 0; x < H; ++x) {
-        uint32_t r[4], k0[4], k1[4];
-        ldmatrix_x4(kt + swizzled<D>(row + 16 * x, 2 * i + half), r[0], r[1], r[2], r[3]);
-        q8::e4m3x4_to_f16x4(r[0], k0[0], k0[2]);
-        q8::e4m3x4_to_f16x4(r[1], k0[1], k0[3]);
-        q8::e4m3x4_to_f16x4(r[2], k1[0], k1[2]);
-        q8::e4m3x4_to_f16x4(r[3], k1[1], k1[3]);
+        float top = fmaxf(s[x][e], s[x][e + 2]);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {  // two chains of products per group: half the latency
-          mma_f16(s[x][n], k0[0], k0[1], k0[2], k0[3], b0[n].x, b0[n].y);
-          mma_f16(s2[x][n], k1[0], k1[1], k1[2], k1[3], b1[n].x, b1[n].y);
-        }
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        m = fmaxf(m, top);
+        M = fmaxf(M, top + lv[x]);
+      }
+      const float fl = ex2(a.m[0][e] - pivot(m)), fo = ex2(a.M[0][e] - pivot(M));
+      a.m[0][e] = m;
+      a.M[0][e] = M;
+      a.l[0][e] *= fl;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        a.o[0][k][e] *= fo;
+        a.o[0][k][e + 2] *= fo;
       }
     }
-    float lv[H];
+  }
+  uint32_t pb[H][2];
+  const float m0 = pivot(a.m[0][0]), m1 = pivot(a.m[0][1]), M0 = pivot(a.M[0][0]), M1 = pivot(a.M[0][1]);
 #pragma unroll
-    for (int x = 0; x < H; ++x) {
-      const bool live = slice + 16 * x < len;  // past the row a scale can be anything
-      const float ks = live ? scales[warp * 2 + s0 + x] : 1.f;
-      lv[x] = live ? log2_scale(scales[kSlices + warp * 2 + s0 + x]) : 0.f;
+  for (int x = 0; x < H; ++x) {
+    a.l[0][0] += ex2(s[x][0] - m0) + ex2(s[x][2] - m0);
+    a.l[0][1] += ex2(s[x][1] - m1) + ex2(s[x][3] - m1);
+    const float f0 = lv[x] - M0, f1 = lv[x] - M1;
+    pb[x][0] = movmatrix_trans(pack_f16x2(ex2(s[x][0] + f0), ex2(s[x][1] + f1)));
+    pb[x][1] = movmatrix_trans(pack_f16x2(ex2(s[x][2] + f0), ex2(s[x][3] + f1)));
+  }
+  if (!tail) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+    for (int x = 0; x < H; ++x) value_product<D>(a.o[0], vt, row + 16 * x, half, kPick, kPick, pb[x]);
+    return;
+  }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][n][e] = (s[x][n][e] + s2[x][n][e]) * (a.qs[n][e & 1] * ks);
+  for (int x = 0; x < H; ++x) {
+    const int left = len - slice - 16 * x;
+    // A NaN in a slot that only some members see: their zero weights must not meet it, so each
+    // member's column is kept from a product of its own, over the slots it sees. Never taken on
+    // sound values.
+    if (p.chain != nullptr && left > 0 && any_nan<D>(vt, row - (lane & 15) + 16 * x, lane)) {
+#pragma unroll 1
+      for (int col = 0; col < p.width; ++col) {
+        const int t = (chunk * p.width + col) / p.groups;
+        bool seen[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          seen[e] = sees(slice + 16 * x + 2 * c + (e & 1) + (e >> 1) * 8, len, position, t, chain);
+        float o[D / 16][4] = {};
+        value_product<D>(o, vt, row + 16 * x, half, pick_slots(seen[0], seen[1]), pick_slots(seen[2], seen[3]), pb[x]);
+        if (col >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          (col & 1 ? a.o[0][k][1] : a.o[0][k][0]) += col & 1 ? o[k][1] : o[k][0];
+          (col & 1 ? a.o[0][k][3] : a.o[0][k][2]) += col & 1 ? o[k][3] : o[k][2];
+        }
+      }
+      continue;
     }
-    // every member sees slots [0, position]; past them the chain rule decides per token
-    const bool tail = slice + 16 * H > (p.chain != nullptr ? position + 1 : len);
-    if (tail) {
+    // slots past the row hold anything, NaN codes too: a zero weight must not meet them
+    value_product<D>(a.o[0], vt, row + 16 * x, half, pick_slots(2 * c < left, 2 * c + 1 < left),
+                     pick_slots(2 * c + 8 < left, 2 * c + 9 < left), pb[x]);
+  }
+}
+
+// More column groups: warp w scores slice w, then multiplies every slice's weights by its 16 dims (with
+// head_dim 64 half of the slices: warps w and w + 4 share dims).
+template <int D, int NG>
+__device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const Smem<D, NG>& sm,
+                                            const float* scales, uint32_t kt, uint32_t vt, int k, bool fresh, int first, int len,
+                                            int position, int chain, int chunk, int warp, int lane) {
+  using S = Smem<D, NG>;
+  const int g = lane >> 2, c = lane & 3;
+  const int slice = first + warp * 16;
+  const int clear = p.chain != nullptr ? position + 1 : len;  // slots that every member sees
+  auto token = [&](int col) { return *reinterpret_cast<const int*>(sm.query + col * S::kQueryPitch + D * 2 + 4); };
+  float s[NG][4];
 #pragma unroll
-      for (int x = 0; x < H; ++x)
+  for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+  float lv = 0.f;
+  if (slice < len) {
+    const int row = warp * 16 + (lane & 15), half = lane >> 4;
+    const uint8_t* query = sm.query + g * S::kQueryPitch + 8 * c;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int slot = slice + 16 * x + g + (e >> 1) * 8;
-            const int t = p.chain != nullptr ? (chunk * p.width + n * 8 + 2 * c + (e & 1)) / p.groups : 0;
-            if (!sees(slot, len, position, t, chain)) s[x][n][e] = -INFINITY;
-          }
+    for (int i = 0; i < D / 32; ++i) {
+      uint32_t r[4], k0[4], k1[4];
+      ldmatrix_x4(kt + swizzled<D>(row, 2 * i + half), r[0], r[1], r[2], r[3]);
+      q8::e4m3x4_to_f16x4(r[0], k0[0], k0[2]);
+      q8::e4m3x4_to_f16x4(r[1], k0[1], k0[3]);
+      q8::e4m3x4_to_f16x4(r[2], k1[0], k1[2]);
+      q8::e4m3x4_to_f16x4(r[3], k1[1], k1[3]);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const uint8_t* src = query + n * 8 * S::kQueryPitch + i * 64;
+        const uint2 b0 = *reinterpret_cast<const uint2*>(src), b1 = *reinterpret_cast<const uint2*>(src + 32);
+        mma_f16(s[n], k0[0], k0[1], k0[2], k0[3], b0.x, b0.y);
+        mma_f16(s[n], k1[0], k1[1], k1[2], k1[3], b1.x, b1.y);
+      }
     }
-    bool moves = false;
+    const float ks = scales[warp];
+    lv = log2_scale(scales[kSlices + warp]);
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 4; ++e) s[n][e] *= a.qs[n][e & 1] * ks;
+  }
+  if (slice + 16 > clear) {
 #pragma unroll
-        for (int x = 0; x < H; ++x)
-          moves = moves || fmaxf(s[x][n][e], s[x][n][e + 2]) > fminf(a.m[n][e], a.M[n][e] - lv[x]) + kSlack;
-    if (__any_sync(0xffffffffu, moves)) {
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int e = 0; e < 4; ++e)
+        if (!sees(slice + g + (e >> 1) * 8, len, position, token(n * 8 + 2 * c + (e & 1)), chain)) s[n][e] = -INFINITY;
+  }
+  bool moves = false;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = a.m[n][e], M = a.M[n][e];
+  for (int n = 0; n < NG; ++n)
 #pragma unroll
-          for (int x = 0; x < H; ++x) {
-            float top = fmaxf(s[x][n][e], s[x][n][e + 2]);
+    for (int e = 0; e < 2; ++e) moves = moves || fmaxf(s[n][e], s[n][e + 2]) > fminf(a.m[n][e], a.M[n][e] - lv) + kSlack;
+  uint2* weights = reinterpret_cast<uint2*>(sm.weights + k % 2 * (S::kWeights / 2)) + lane;
+  // weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile
+  for (;; fresh = moves = false) {
+    if (!fresh) {
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            m = fmaxf(m, top);
-            M = fmaxf(M, top + lv[x]);
-          }
-          const float fl = ex2(a.m[n][e] - pivot(m)), fo = ex2(a.M[n][e] - pivot(M));
-          a.m[n][e] = m;
-          a.M[n][e] = M;
-          a.l[n][e] *= fl;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            a.o[n][k][e] *= fo;
-            a.o[n][k][e + 2] *= fo;
-          }
-        }
+      for (int n = 0; n < NG; ++n) {
+        const float f0 = lv - pivot(a.M[n][0]), f1 = lv - pivot(a.M[n][1]);
+        const uint32_t lo = movmatrix_trans(pack_f16x2(ex2(s[n][0] + f0), ex2(s[n][1] + f1)));
+        const uint32_t hi = movmatrix_trans(pack_f16x2(ex2(s[n][2] + f0), ex2(s[n][3] + f1)));
+        weights[(warp * NG + n) * 32] = make_uint2(lo, hi);
     }
-    uint32_t pb[H][NG][2];
+      if (!consumers_any<NG>(moves)) break;
+    }
+    // [warp][column], where the last tile's weights were: everyone has multiplied by them (a run's first
+    // tile: start_unit)
+    float2* tops = reinterpret_cast<float2*>(sm.weights + (k + 1) % 2 * (S::kWeights / 2));
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      const float m0 = pivot(a.m[n][0]), m1 = pivot(a.m[n][1]), M0 = pivot(a.M[n][0]), M1 = pivot(a.M[n][1]);
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int x = 0; x < H; ++x) {
-        a.l[n][0] += ex2(s[x][n][0] - m0) + ex2(s[x][n][2] - m0);
-        a.l[n][1] += ex2(s[x][n][1] - m1) + ex2(s[x][n][3] - m1);
-        const float f0 = lv[x] - M0, f1 = lv[x] - M1;
-        pb[x][n][0] = movmatrix_trans(pack_f16x2(ex2(s[x][n][0] + f0), ex2(s[x][n][1] + f1)));
-        pb[x][n][1] = movmatrix_trans(pack_f16x2(ex2(s[x][n][2] + f0), ex2(s[x][n][3] + f1)));
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (g == 0) tops[warp * NG * 8 + n * 8 + 2 * c + e] = make_float2(top, top + lv);
+      }
+    consumers_sync<NG>();
+    float2 top = make_float2(-INFINITY, -INFINITY);  // of column `lane`
+    if (lane < NG * 8) {
+#pragma unroll
+      for (int w = 0; w < kConsumers<NG>; ++w) {
+        const float2 t = tops[w * NG * 8 + lane];
+        top = make_float2(fmaxf(top.x, t.x), fmaxf(top.y, t.y));
       }
     }
-    if (!tail) {
 #pragma unroll
-      for (int x = 0; x < H; ++x) value_product<D, NG>(a.o, vt, row + 16 * x, half, kPick, kPick, pb[x]);
-      continue;
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float m = fmaxf(a.m[n][e], __shfl_sync(0xffffffffu, top.x, n * 8 + 2 * c + e));
+        const float M = fmaxf(a.M[n][e], __shfl_sync(0xffffffffu, top.y, n * 8 + 2 * c + e));
+        const float fl = ex2(a.m[n][e] - pivot(m)), fo = ex2(a.M[n][e] - pivot(M));
+        a.m[n][e] = m;
+        a.M[n][e] = M;
+        a.l[n][e] *= fl;
+        a.o[n][0][e] *= fo;
+        a.o[n][0][e + 2] *= fo;
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const float m0 = pivot(a.m[n][0]), m1 = pivot(a.m[n][1]);
+    a.l[n][0] += ex2(s[n][0] - m0) + ex2(s[n][2] - m0);
+    a.l[n][1] += ex2(s[n][1] - m1) + ex2(s[n][3] - m1);
+  }
+  constexpr int kChunks = D / 16, kShare = kSlices * kChunks / kConsumers<NG>;
+  const int dims = warp % kChunks, from = warp / kChunks * kShare;
+  if (first + kTile <= clear) {
+#pragma unroll
+    for (int y0 = 0; y0 < kShare; y0 += 2) {
+      uint32_t r[4];
+      ldmatrix_x4_trans(vt + swizzled<D>(16 * (from + y0) + lane, dims), r[0], r[1], r[2], r[3]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t f[4];
+        value_fragments(f, r[2 * x], r[2 * x + 1], kPick, kPick);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const uint2 pb = weights[((from + y0 + x) * NG + n) * 32];
+          mma_f16(a.o[n][0], f[0], f[1], f[2], f[3], pb.x, pb.y);
+        }
+      }
     }
+    return;
+  }
+  // the row's last tiles; kept small, since their code shares the instruction cache with the loop above
+#pragma unroll 1
+  for (int y = from; y < from + kShare; ++y) {
+    const int at = first + 16 * y, left = len - at;
+    if (left <= 0) break;
+    uint32_t r[4], f[4];
+    ldmatrix_x4_trans(vt + swizzled<D>(16 * y + (lane & 15), dims), r[0], r[1], r[2], r[3]);  // twice the slice
+    bool nan = false;
+    if (at + 16 > clear && p.chain != nullptr && lane < 16 && lane < left) {
+      const uint32_t src = vt + swizzled<D>(16 * y + lane, dims);
 #pragma unroll
-    for (int x = 0; x < H; ++x) {
-      const int left = len - slice - 16 * x;
-      // A NaN in a slot that only some members see: their zero weights must not meet it, so each
-      // member's column is kept from a product of its own, over the slots it sees. Never taken on
-      // sound values.
-      if (p.chain != nullptr && left > 0 && any_nan<D>(vt, row - (lane & 15) + 16 * x, lane)) {
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(src + 4 * i) : "memory");
+        nan = nan || has_nan(w);
+      }
+    }
+    if (__any_sync(0xffffffffu, nan)) {
+      // A NaN in a slot that only some members see: as above, a product for each of them.
+#pragma unroll 1
+      for (int col = 0; col < p.width; ++col) {
+        const int t = token(col), group = col / 8;
+        bool seen[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen[e] = sees(at + 2 * c + (e & 1) + (e >> 1) * 8, len, position, t, chain);
+        value_fragments(f, r[0], r[1], pick_slots(seen[0], seen[1]), pick_slots(seen[2], seen[3]));
+        const uint2 pb = weights[(y * NG + group) * 32];
+        float o[4] = {};
+        mma_f16(o, f[0], f[1], f[2], f[3], pb.x, pb.y);
+        if ((col & 7) >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
 #pragma unroll
         for (int n = 0; n < NG; ++n)
-#pragma unroll 1
-          for (int col = 0; col < 8 && n * 8 + col < p.width; ++col) {
-            const int t = (chunk * p.width + n * 8 + col) / p.groups;
-            bool seen[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              seen[e] = sees(slice + 16 * x + 2 * c + (e & 1) + (e >> 1) * 8, len, position, t, chain);
-            const uint32_t one[1][2] = {{pb[x][n][0], pb[x][n][1]}};
-            float o[1][D / 16][4] = {};
-            value_product<D, 1>(o, vt, row + 16 * x, half, pick_slots(seen[0], seen[1]), pick_slots(seen[2], seen[3]), one);
-            if (col >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              (col & 1 ? a.o[n][k][1] : a.o[n][k][0]) += col & 1 ? o[0][k][1] : o[0][k][0];
-              (col & 1 ? a.o[n][k][3] : a.o[n][k][2]) += col & 1 ? o[0][k][3] : o[0][k][2];
-            }
+          if (n == group) {
+            a.o[n][0][0] += col & 1 ? 0.f : o[0];
+            a.o[n][0][1] += col & 1 ? o[1] : 0.f;
+            a.o[n][0][2] += col & 1 ? 0.f : o[2];
+            a.o[n][0][3] += col & 1 ? o[3] : 0.f;
           }
-        continue;
       }
-      // slots past the row hold anything, NaN codes too: a zero weight must not meet them
-      value_product<D, NG>(a.o, vt, row + 16 * x, half, pick_slots(2 * c < left, 2 * c + 1 < left),
-                           pick_slots(2 * c + 8 < left, 2 * c + 9 < left), pb[x]);
+      continue;
+    }
+    // slots past the row hold anything, NaN codes too: a zero weight must not meet them
+    value_fragments(f, r[0], r[1], pick_slots(2 * c < left, 2 * c + 1 < left),
+                    pick_slots(2 * c + 8 < left, 2 * c + 9 < left));
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const uint2 pb = weights[(y * NG + n) * 32];
+      mma_f16(a.o[n][0], f[0], f[1], f[2], f[3], pb.x, pb.y);
     }
   }
 }
 
-// Sums the consumer warps' states in warp order, column group by column group: sink(in_chunk, d, O, M,
-// m, l) for every live column and dim.
-template <int D, int NG, typename Sink>
-__device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, float* red_stats, int members, int warp,
-                                             int lane, Sink sink) {
+// Sums the consumer warps' states in warp order: sink(in_chunk, d, O, M, m, l) for every live column and
+// dim.
+template <int D, typename Sink>
+__device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& sm, int members, int warp, int lane,
+                                             Sink sink) {
+  constexpr int NG = 1, kWarps = kConsumers<1>;
+  float *red_o = sm.red_o, *red_stats = sm.red_stats;
   const int g = lane >> 2, c = lane & 3, tid = threadIdx.x;
 #pragma unroll
   for (int n = 0; n < NG; ++n)
@@ -484,17 +667,17 @@ __device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, floa
       }
     }
 #pragma unroll
-  for (int pass = 0; pass < 2 * NG; ++pass) {
-    const int n = pass / 2, k0 = pass % 2 * (D / 32);  // column group, half of its dims
-    if (n * 8 >= members) break;                       // uniform
-    if (pass > 0) consumers_sync();                    // the last pass's reads are done
+  for (int pass = 0; pass < 2; ++pass) {  // half of the dims each
+    constexpr int n = 0;
+    const int k0 = pass * (D / 32);
+    if (pass > 0) consumers_sync<NG>();  // the last pass's reads are done
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       float* dst = red_o + (warp * (D / 2) + 16 * k + 2 * g) * 8 + 2 * c;
       *reinterpret_cast<float2*>(dst) = make_float2(a.o[n][k0 + k][0], a.o[n][k0 + k][1]);
       *reinterpret_cast<float2*>(dst + 8) = make_float2(a.o[n][k0 + k][2], a.o[n][k0 + k][3]);
     }
-    consumers_sync();
+    consumers_sync<NG>();
 #pragma unroll
     for (int e0 = 0; e0 < 8 * (D / 2); e0 += kWarps * 32) {
       const int e = e0 + tid, col = e / (D / 2), d = e % (D / 2), in_chunk = n * 8 + col;
@@ -517,18 +700,85 @@ __device__ __forceinline__ void reduce_warps(State<D, NG>& a, float* red_o, floa
   }
 }
 
+// More column groups: what the warps tell each other after `k` tiles, where the next tile's weights would go.
+template <int D, int NG>
+struct Totals {
+  float* l;        // [warp][column]: denominators of the warp's slices
+  float2* pivots;  // [column]: M, m
+  float4* stats;   // [column]: M, m, l
+  __device__ Totals(const Smem<D, NG>& sm, int k) {
+    l = reinterpret_cast<float*>(sm.weights + k % 2 * (Smem<D, NG>::kWeights / 2));
+    pivots = reinterpret_cast<float2*>(l + kConsumers<NG> * NG * 8);
+    stats = reinterpret_cast<float4*>(pivots + NG * 8);
+  }
+  // A column's M, m and l, summed in warp order.
+  __device__ float4 column(int col) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kConsumers<NG>; ++w) sum += l[w * NG * 8 + col];
+    return make_float4(pivots[col].x, pivots[col].y, sum, 0.f);
+  }
+};
+
+// Each warp ends with O of its dims; with head_dim 64 the first of the two that share dims.
+template <int D, int NG>
+__device__ __forceinline__ void join_warps(State<D, NG>& a, const Smem<D, NG>& sm, const Totals<D, NG>& totals, int warp,
+                                           int lane) {
+  constexpr int kChunks = D / 16;
+  const int g = lane >> 2, c = lane & 3;
+  float4* other = reinterpret_cast<float4*>(sm.red_o) + warp % kChunks * NG * 32 + lane;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = n * 8 + 2 * c + e;
+      float l = a.l[n][e];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      if (g == 0) totals.l[warp * NG * 8 + col] = l;
+      if (g == 0 && warp == 0) totals.pivots[col] = make_float2(a.M[n][e], a.m[n][e]);
+    }
+    if (warp >= kChunks) other[n * 32] = make_float4(a.o[n][0][0], a.o[n][0][1], a.o[n][0][2], a.o[n][0][3]);
+  }
+  consumers_sync<NG>();
+  if (kChunks < kConsumers<NG> && warp < kChunks) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const float4 v = other[n * 32];
+      a.o[n][0][0] += v.x, a.o[n][0][1] += v.y, a.o[n][0][2] += v.z, a.o[n][0][3] += v.w;
+    }
+  }
+}
+
+// sink(column, dim, value, value of the next dim) for the live columns of this thread.
+template <int D, int NG, typename Sink>
+__device__ __forceinline__ void each_pair(const State<D, NG>& a, int members, int warp, int lane, Sink sink) {
+  if (warp >= D / 16) return;
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = n * 8 + 2 * (lane & 3) + e;
+      if (col < members) sink(col, 16 * warp + 2 * (lane >> 2), a.o[n][0][e], a.o[n][0][e + 2]);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ __nv_bfloat16* out_row(const Params& p, int b, int h, int member) {
+  const int t = member / p.groups, head = h * p.groups + member - t * p.groups;
+  return p.out + ((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D;
+}
 template <int D>
 __device__ __forceinline__ void write_out(const Params& p, int b, int h, int member, int d, float O, float M, float m,
                                           float l) {
-  const int t = member / p.groups, head = h * p.groups + member - t * p.groups;
-  p.out[((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D + d] = __float2bfloat16_rn(finished(O, M, m, l));
+  out_row<D>(p, b, h, member)[d] = __float2bfloat16_rn(finished(O, M, m, l));
 }
 
 template <int D, int NG>
 __device__ __forceinline__ void init_barriers(const Smem<D, NG>& sm, const CUtensorMap* kmap, const CUtensorMap* vmap) {
   for (int s = 0; s < Smem<D, NG>::kStages; ++s) {
     mbar_init(&sm.full[s], 1 + kScales);  // the tiles' bytes and the scale copies
-    mbar_init(&sm.empty[s], kWarps);
+    mbar_init(&sm.empty[s], kConsumers<NG>);
   }
   fence_barrier_init();
   prefetch_tensormap(kmap);
@@ -577,7 +827,7 @@ __device__ __forceinline__ void drain(const Smem<D, NG>& sm, int issued) {
 // Consumer warp: tile j of a row with `len` slots from stage k % stages. After an abort the barriers
 // that follow are still taken, on whatever the stage holds.
 template <int D, int NG>
-__device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>& sm, const Params& p, int k, int j,
+__device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>& sm, const Params& p, int k, bool fresh, int j,
                                              int len, int position, int chain, int chunk, int warp, int lane) {
   using S = Smem<D, NG>;
   const int s = k % S::kStages;
@@ -587,8 +837,8 @@ __device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>&
   }
   __syncwarp();
   const uint32_t kt = smem_u32(sm.ring + s * 2 * S::kTileBytes);
-  attend_tile<D, NG>(a, p, sm.query, sm.scales + s * kScales, kt, kt + S::kTileBytes, j * kTile, len, position, chain,
-                     chunk, warp, lane);
+  attend_tile(a, p, sm, sm.scales + s * kScales, kt, kt + S::kTileBytes, k, fresh, j * kTile, len, position, chain, chunk, warp,
+              lane);
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.empty[s]);
 }
@@ -599,11 +849,12 @@ __device__ __forceinline__ int first_position(const Params& p, int b) {
 
 // ------------------------------------------------------------------------------ cluster form
 template <int D, int NG>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads<NG>, 2)
     cluster_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                    const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   const Smem<D, NG> sm(smem_raw);
+  constexpr int kWarps = kConsumers<NG>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = gridDim.x, rank = blockIdx.x;  // cluster dims (C, 1, 1)
   const int pair = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks;
@@ -630,45 +881,87 @@ __global__ void __launch_bounds__(kThreads, 2)
   State<D, NG> a;
   start_unit<D, NG>(a, p, sm.query, b, h, chunk, warp, lane);
   for (int k = 0; k < count; ++k)
-    consume_tile(a, sm, p, k, rank + k * C, len, position, chain, chunk, warp, lane);
-  const int total = members * D, share = (total + C - 1) / C;
-  cluster_wait();  // every CTA of the cluster runs
-  reduce_warps<D, NG>(a, sm.red_o, sm.red_stats, members, warp, lane,
-                      [&](int col, int d, float O, float M, float m, float l) {
-                        const int e = col * D + d, owner = e / share;
-                        st_cluster_f32(map_shared(smem_u32(sm.recv_o + rank * share + e - owner * share), owner), O);
-                        if (d < C) {  // one thread per rank passes this column's statistics on
-                          const uint32_t at = map_shared(smem_u32(sm.recv_stats + (rank * NG * 8 + col) * 3), d);
-                          st_cluster_f32(at, M);
-                          st_cluster_f32(at + 4, m);
-                          st_cluster_f32(at + 8, l);
-                        }
-                      });
+    consume_tile(a, sm, p, k, k == 0, rank + k * C, len, position, chain, chunk, warp, lane);
+  // values of an owner: an even number, so that pairs stay together; e / share for e < 2^16
+  const int total = members * D, share = (total + 2 * C - 1) / (2 * C) * 2;
+  const uint32_t magic = (0xffffffffu / share) + 1;
+  auto push_stats = [&](int col, int to, float M, float m, float l) {
+    const uint32_t at = map_shared(smem_u32(sm.recv_stats + (rank * NG * 8 + col) * 3), to);
+    st_cluster_f32(at, M);
+    st_cluster_f32(at + 4, m);
+    st_cluster_f32(at + 8, l);
+  };
+  auto push_to = [&](int e) {
+    const int owner = __umulhi(e, magic);
+    return map_shared(smem_u32(sm.recv_o + rank * share + e - owner * share), owner);
+  };
+  if constexpr (NG == 1) {
+    cluster_wait();  // every CTA of the cluster runs
+    reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float M, float m, float l) {
+      st_cluster_f32(push_to(col * D + d), O);
+      if (d < C) push_stats(col, d, M, m, l);  // one thread per rank passes this column's statistics on
+    });
+  } else {
+    const Totals<D, NG> totals(sm, count);
+    join_warps(a, sm, totals, warp, lane);
+    cluster_wait();  // every CTA of the cluster runs
+    each_pair(a, members, warp, lane, [&](int col, int d, float O0, float O1) {
+      st_cluster_f32x2(push_to(col * D + d), O0, O1);
+    });
+    if (lane < members) {
+      const float4 st = totals.column(lane);
+      for (int to = warp; to < C; to += kWarps) push_stats(lane, to, st.x, st.y, st.z);
+    }
+  }
   cluster_sync();  // every partial has landed; nobody touches another CTA's memory after this
+  // a rank's weight in a column's output, in place of its M; a column that sees nothing, or only zero
+  // values, is marked by l = 0
+  for (int c0 = 0; c0 < NG * 8; c0 += kWarps * 2) {
+    const int col = c0 + static_cast<int>(threadIdx.x) / 16, q = threadIdx.x & 15;
+    static_assert(kMaxCluster == 16, "a rank per lane of half a warp");
+    const bool on = col < members && q < C;
+    float* st = sm.recv_stats + (q * NG * 8 + col) * 3;
+    const float M_q = on ? st[0] : -INFINITY, m_q = on ? st[1] : -INFINITY;
+    float M = M_q, m = m_q;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    }
+    float l = on ? st[2] * ex2(m_q - pivot(m)) : 0.f;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (on) {
+      st[0] = ex2(M_q - pivot(M)) * finished(1.f, M, m, l);
+      st[2] = M == -INFINITY && l > 0.f ? 0.f : l;
+    }
+  }
+  consumers_sync<NG>();
   const int low = rank * share, high = min(total, low + share);
-  for (int e = low + static_cast<int>(threadIdx.x); e < high; e += kWarps * 32) {
+  for (int e = low + 2 * static_cast<int>(threadIdx.x); e < high; e += 2 * kWarps * 32) {
     const int col = e / D;
-    float M = -INFINITY, m = -INFINITY, O = 0.f, l = 0.f;
+    const float* st = sm.recv_stats + col * 3;
+    float O0 = 0.f, O1 = 0.f;
     for (int q = 0; q < C; ++q) {
-      M = fmaxf(M, sm.recv_stats[(q * NG * 8 + col) * 3]);
-      m = fmaxf(m, sm.recv_stats[(q * NG * 8 + col) * 3 + 1]);
+      const float2 v = *reinterpret_cast<const float2*>(sm.recv_o + q * share + e - low);
+      const float w = st[q * NG * 8 * 3];
+      O0 += v.x * w;
+      O1 += v.y * w;
     }
-    for (int q = 0; q < C; ++q) {
-      const float* st = sm.recv_stats + (q * NG * 8 + col) * 3;
-      O += sm.recv_o[q * share + e - low] * ex2(st[0] - pivot(M));
-      l += st[2] * ex2(st[1] - pivot(m));
-    }
-    write_out<D>(p, b, h, chunk * p.width + col, e % D, O, M, m, l);
+    const bool none = st[2] == 0.f;
+    *reinterpret_cast<__nv_bfloat162*>(out_row<D>(p, b, h, chunk * p.width + col) + e % D) =
+        __floats2bfloat162_rn(none ? 0.f : O0, none ? 0.f : O1);
   }
 }
 
 // --------------------------------------------------------------------------- persistent form
 template <int D, int NG>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads<NG>, 2)
     persistent_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   const Smem<D, NG> sm(smem_raw);
+  constexpr int kWarps = kConsumers<NG>;
   const int* cum = sm.cum;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int B = p.batch, per_row = p.kv_heads * p.chunks;  // units of a row
@@ -745,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       run_first = j;
       start_unit<D, NG>(a, p, sm.query, b, u / p.chunks, u % p.chunks, warp, lane);
     }
-    consume_tile(a, sm, p, k, j, len, position, chain, u % p.chunks, warp, lane);
+    consume_tile(a, sm, p, k, starts, j, len, position, chain, u % p.chunks, warp, lane);
     const int run_b = b, run_u = u, run_last = j;
     starts = k == count - 1;
     if (++j == n) {
@@ -762,16 +1055,38 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int h = run_u / p.chunks, chunk = run_u % p.chunks;
     const size_t slot = blockIdx.x + static_cast<size_t>(run_b) * per_row + run_u;
     const bool whole = run_first == 0 && run_last == n - 1;
-    consumers_sync();  // the last run's reductions are read
-    reduce_warps<D, NG>(a, sm.red_o, sm.red_stats, min(p.width, p.members - chunk * p.width), warp, lane,
-                        [&](int col, int d, float O, float M, float m, float l) {
-                          if (whole) {
-                            write_out<D>(p, run_b, h, chunk * p.width + col, d, O, M, m, l);
-                          } else {
-                            p.acc[(slot * p.width + col) * D + d] = O;
-                            if (d == 0) p.stats[slot * p.width + col] = make_float4(M, m, l, 0.f);
-                          }
-                        });
+    const int members = min(p.width, p.members - chunk * p.width);
+    if constexpr (NG == 1) {
+      consumers_sync<NG>();  // the last run's reductions are read
+      reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float M, float m, float l) {
+        if (whole) {
+          write_out<D>(p, run_b, h, chunk * p.width + col, d, O, M, m, l);
+        } else {
+          p.acc[(slot * p.width + col) * D + d] = O;
+          if (d == 0) p.stats[slot * p.width + col] = make_float4(M, m, l, 0.f);
+        }
+      });
+    } else {
+      const Totals<D, NG> totals(sm, k + 1);
+      join_warps(a, sm, totals, warp, lane);
+      if (warp == 0 && lane < members) {
+        const float4 st = totals.column(lane);
+        if (whole)
+          totals.stats[lane] = st;
+        else
+          p.stats[slot * p.width + lane] = st;
+      }
+      if (whole) consumers_sync<NG>();
+      each_pair(a, members, warp, lane, [&](int col, int d, float O0, float O1) {
+        if (whole) {
+          const float4 st = totals.stats[col];
+          *reinterpret_cast<__nv_bfloat162*>(out_row<D>(p, run_b, h, chunk * p.width + col) + d) = __floats2bfloat162_rn(
+              finished(O0, st.x, st.y, st.z), finished(O1, st.x, st.y, st.z));
+        } else {
+          *reinterpret_cast<float2*>(p.acc + (slot * p.width + col) * D + d) = make_float2(O0, O1);
+        }
+      });
+    }
   }
 }
 
@@ -846,12 +1161,11 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   }
 }
 
-// Columns of a unit: the least number of equal member groups of at most 24 (D = 128: the
-// accumulators of 32 would not fit the registers) or 32 columns.
-void chunk_members(Params* p, int head_dim) {
-  const int most = head_dim == 128 ? 24 : 32;
+// Columns of a unit: the least number of equal member groups of at most 32 columns.
+void chunk_members(Params* p) {
+  constexpr int kMost = 32;
   p->members = p->tokens * p->groups;
-  p->chunks = (p->members + most - 1) / most;
+  p->chunks = (p->members + kMost - 1) / kMost;
   p->width = (p->members + p->chunks - 1) / p->chunks;
   p->chunks = (p->members + p->width - 1) / p->width;
 }
@@ -883,7 +1197,7 @@ int shape(Params* p, const fb_q8_cache& cache, int tokens, int q_heads) {
   p->block = block;
   p->blocks = (capacity + block - 1) / block;
   p->ctas = 2 * sm_count();
-  chunk_members(p, head_dim);
+  chunk_members(p);
   const long long row_units = static_cast<long long>(kv_heads) * p->chunks;
   return batch * row_units >= (1ll << 31) || row_units * tiles_of(capacity) >= (1ll << 31) ? FB_ERR_SHAPE : FB_OK;
 }
@@ -915,7 +1229,7 @@ int resident_clusters(int c) {
   if (dev < kMaxDevices && cache[dev][c] != 0) return cache[dev][c] - 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c, 1);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreads<NG>);
   cfg.dynamicSmemBytes = Smem<D, NG>::kTotal;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -950,8 +1264,8 @@ int launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int cl
   const int units = p.batch * p.kv_heads * p.chunks;
   constexpr int bytes = Smem<D, NG>::kTotal;
   if (cluster > 0)
-    return launch_ex(cluster_kernel<D, NG>, dim3(cluster, units), dim3(kThreads), bytes, stream, cluster, km, vm, p);
-  const int st = launch_ex(persistent_kernel<D, NG>, dim3(p.ctas), dim3(kThreads), bytes, stream, 1, km, vm, p);
+    return launch_ex(cluster_kernel<D, NG>, dim3(cluster, units), dim3(kThreads<NG>), bytes, stream, cluster, km, vm, p);
+  const int st = launch_ex(persistent_kernel<D, NG>, dim3(p.ctas), dim3(kThreads<NG>), bytes, stream, 1, km, vm, p);
   if (st != FB_OK) return st;
   return launch_ex(merge_kernel<D>, dim3(units, (p.width + 7) / 8), dim3(kMergeThreads), 0, stream, 1, p);
 }
@@ -962,8 +1276,8 @@ auto with_groups(const Params& p, F f) {
   using std::integral_constant;
   if (p.width <= 8) return f(integral_constant<int, D>(), integral_constant<int, 1>());
   if (p.width <= 16) return f(integral_constant<int, D>(), integral_constant<int, 2>());
-  if (D == 128 || p.width <= 24) return f(integral_constant<int, D>(), integral_constant<int, 3>());
-  return f(integral_constant<int, D>(), integral_constant<int, D == 64 ? 4 : 3>());
+  if (p.width <= 24) return f(integral_constant<int, D>(), integral_constant<int, 3>());
+  return f(integral_constant<int, D>(), integral_constant<int, 4>());
 }
 template <typename F>
 auto with_shape(const Params& p, int head_dim, F f) {
@@ -998,7 +1312,7 @@ extern "C" int fb_attention_q8(const void* q, const fb_q8_cache* cache, const in
   int st = attn8::shape(&p, *cache, tokens, q_heads);
   if (st != FB_OK) return st;
   if ((chain == nullptr && tokens != 1) || (chain != nullptr && !per_row)) return FB_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(q) & 7u) != 0) return FB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) & 7u) != 0 || (reinterpret_cast<uintptr_t>(out) & 3u) != 0) return FB_ERR_ARG;
   const int head_dim = cache->head_dim;
   const int cluster = attn8::plan(p, head_dim);
   if (cluster < 0) return cluster;

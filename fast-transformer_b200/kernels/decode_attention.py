@@ -121,12 +121,14 @@ def block_attention(query, key, value, position, scale, chain, splits=None):
 
 def _attend_q8(query, cache, position, per_row, chain, tokens, q_heads, shape, scale):
     device = cache.device
-    if query.device != device or position.device != device or (chain is not None and chain.device != device):
+    index = device.index
+    if query.get_device() != index or position.get_device() != index or (
+            chain is not None and chain.get_device() != index):
         raise ValueError(f"8-bit attention takes tensors on the cache's device, {device}")
     assert query.dtype == torch.bfloat16 and query.is_contiguous()
     assert position.dtype == torch.int64 and position.is_contiguous()
     need = cache.workspace_bytes(tokens, q_heads)
-    out = query.new_empty(shape)
+    out = query.new_empty(*shape)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     launch("fb_attention_q8", device, query.data_ptr(), cache.address, position.data_ptr(), per_row,
            None if chain is None else chain.data_ptr(), out.data_ptr(), workspace.data_ptr() if need else None, need,

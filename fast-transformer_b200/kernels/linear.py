@@ -102,9 +102,9 @@ def _project4(flat, weight, epilogue):
     if epilogue == SWIGLU_OUT:
         if n % 128:
             raise ValueError(f"SwiGLU weights are 64-row gate/up blocks: {n} rows are not a multiple of 128")
-        out = flat.new_empty((m, n // 2))
+        out = flat.new_empty(m, n // 2)
     elif epilogue == BF16_OUT:
-        out = flat.new_empty((m, n))
+        out = flat.new_empty(m, n)
     else:
         out = flat.new_empty((1, m, n) if epilogue == SPLITS_OUT else (m, n), dtype=torch.float32)
     return _launch4(flat.contiguous(), weight, out, m, FP32_OUT if epilogue == SPLITS_OUT else epilogue)
@@ -118,7 +118,7 @@ def _linear4(x, weight):
     if rows > MAX_ROWS:
         _native.require_device(weight.device, x)
         return F.linear(x, weight.dequantized())
-    out = x.new_empty((*shape[:-1], weight.n))
+    out = x.new_empty(*shape[:-1], weight.n)
     return _launch4(x if x.is_contiguous() else x.contiguous(), weight, out, rows, BF16_OUT) if rows else out
 
 

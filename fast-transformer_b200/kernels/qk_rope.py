@@ -80,11 +80,14 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, cache, q_heads,
     q_weight, k_weight = q_norm.weight, k_norm.weight
     assert q_weight.dtype == k_weight.dtype == torch.bfloat16 and q_weight.numel() == k_weight.numel() == dim
     assert q_weight.is_contiguous() and k_weight.is_contiguous()
-    _native.require_device(device, data, cos, sin, position, phases, q_weight, k_weight)
-    query = cos.new_empty((batch, tokens, q_heads, dim))
+    if not (data.get_device() == cos.get_device() == sin.get_device() == position.get_device() ==
+            q_weight.get_device() == k_weight.get_device() == device.index) or phases is not None:
+        _native.require_device(device, data, cos, sin, position, phases, q_weight, k_weight)
+    token = q_heads * dim  # token-major, seen as [B, Hq, T, D]
+    query = cos.new_empty_strided((batch, q_heads, tokens, dim), (tokens * token, dim, token, 1))
     _native.launch(
         "fb_qk_norm_rope_append_q8", device, data.data_ptr(), splits, q_weight.data_ptr(), k_weight.data_ptr(),
         q_norm.variance_epsilon, k_norm.variance_epsilon, cos.data_ptr(), sin.data_ptr(), position.data_ptr(),
         None if phases is None else phases.data_ptr(), query.data_ptr(), cache.address, tokens, q_heads,
         1 if prefill else 2 if rows else 0, 1 if whole else 0)
-    return query.transpose(1, 2)
+    return query
