@@ -122,15 +122,27 @@ __device__ __forceinline__ void load_packed8(const AppendParams& p, size_t off, 
   for (int e = 0; e < kE; ++e) x[e] = bf16_round(x[e]);
 }
 
-// RMSNorm + RoPE of the rows on a warp, in place, in fp32: w = x * inv * gain, out = w cos + rot(w) sin.
+// gain * cos and the partner's gain * sin of a lane's dims: RoPE of x * inv * gain is then
+// inv * (x c -+ partner s).
+struct Rotation {
+  float c[kE], s[kE];
+  __device__ __forceinline__ Rotation(const uint4& gain, const uint4& cos, const uint4& sin) {
+    float g[kE];
+    unpack8(gain, g);
+    unpack8(cos, c);
+    unpack8(sin, s);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      c[e] *= g[e];
+      s[e] *= g[e ^ 4];
+    }
+  }
+};
+
+// RMSNorm + RoPE of the rows on a warp, in place, in fp32.
 template <int D>
-__device__ __forceinline__ void norm_rope_fp32(float (&x)[kE], const uint4& gain, float eps, const uint4& cos,
-                                               const uint4& sin, int lane) {
+__device__ __forceinline__ void norm_rope_fp32(float (&x)[kE], float eps, const Rotation& r) {
   constexpr int kLanes = Lanes<D>::kLanes;
-  float g[kE], cs[kE], sn[kE];
-  unpack8(gain, g);
-  unpack8(cos, cs);
-  unpack8(sin, sn);
   float ss = 0.f;
 #pragma unroll
   for (int e = 0; e < kE; ++e) ss += x[e] * x[e];
@@ -139,9 +151,9 @@ __device__ __forceinline__ void norm_rope_fp32(float (&x)[kE], const uint4& gain
   const float inv = __frsqrt_rn(ss / static_cast<float>(D) + eps);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float low = x[e] * inv * g[e], high = x[e + 4] * inv * g[e + 4];
-    x[e] = low * cs[e] - high * sn[e];
-    x[e + 4] = high * cs[e + 4] + low * sn[e + 4];
+    const float low = x[e] * inv, high = x[e + 4] * inv;
+    x[e] = low * r.c[e] - high * r.s[e];
+    x[e + 4] = high * r.c[e + 4] + low * r.s[e + 4];
   }
 }
 
@@ -190,13 +202,12 @@ __device__ __forceinline__ float finite_max(const float (&x)[kE], float so_far) 
   return so_far;
 }
 
-// What a launch does: both parts (a decode step: one launch), or, for a prompt, Q heads and blocks in
-// launches of their own, each at the occupancy that its registers allow (one launch of both: 75 us
-// for 8192 tokens of 32 + 8 heads of 128, two: 55 us).
-enum Part : int { kBoth = 0, kQueries = 1, kBlocks = 2 };
-
-template <int D, bool kSplit, int kPart>
-__global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart == kQueries ? 4 : 3) append_kernel(const AppendParams p) {
+// One launch does both. A decode step's CTAs of Q heads come first; a prompt's CTAs of either kind are spread
+// evenly, so that the blocks' chains of loads, norm, barrier and stores hide behind the Q heads' bytes
+// (8192 tokens of 32 + 8 heads of 128: 42.7 us, 4.4 TB/s; a launch of each kind 50.3; 48.9 with all cos and
+// sin loaded at once, three CTAs per SM instead of four).
+template <int D, bool kSplit, bool kPrompt>
+__global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_kernel(const AppendParams p) {
   constexpr int kLanes = Lanes<D>::kLanes, kRows = Lanes<D>::kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane / kLanes, d0 = lane % kLanes * 4;
@@ -205,9 +216,17 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
   pdl_wait();
   pdl_trigger();
 
-  if (kPart != kBlocks && static_cast<int>(blockIdx.x) < p.query_ctas) {
+  const int cta = static_cast<int>(blockIdx.x);
+  int block_cta = cta - p.query_ctas;  // the CTA's number among those with blocks
+  bool takes_block = block_cta >= 0;
+  if (kPrompt) {
+    const long long block_ctas = gridDim.x - p.query_ctas;
+    block_cta = static_cast<int>(cta * block_ctas / gridDim.x);  // CTAs with blocks before this one
+    takes_block = (cta + 1) * block_ctas / gridDim.x > block_cta;
+  }
+  if (!takes_block) {
     // ---- query_heads heads of one token, kRows side by side ----
-    const unsigned item = blockIdx.x * kWarps + warp;  // < 2^31 + kWarps
+    const unsigned item = static_cast<unsigned>(kPrompt ? cta - block_cta : cta) * kWarps + warp;  // < 2^31 + kWarps
     const unsigned nth_row = item / p.runs;
     const int head0 = static_cast<int>(item - nth_row * p.runs) * p.query_heads;
     if (nth_row >= static_cast<unsigned>(p.batch * p.tokens)) return;
@@ -216,11 +235,19 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
     constexpr int kMost = 4;  // loads in flight
     const size_t in = static_cast<size_t>(row) * width + head0 * D + d0;
     __nv_bfloat16* out = p.query + (static_cast<size_t>(row) * p.q_heads + head0) * D + d0;
-    const size_t phase = static_cast<size_t>(phase_row(p, b, t, first_slot(p, b))) * D + d0;
-    const uint4 gain = load8<D>(p.q_weight + d0), cos = load8<D>(p.cos + phase), sin = load8<D>(p.sin + phase);
     // rows of lanes past the last head repeat it and store nothing
+    uint4 raw[kMost];  // the first heads', on their way before the position and its phase are known
+    auto load = [&](int h0) {
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.packed) + in;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+        raw[i] = load8<D>(src + static_cast<size_t>(min(h0 + i * kRows + sub, heads - 1)) * D);
+    };
+    if (!kSplit) load(0);
+    const size_t phase = static_cast<size_t>(phase_row(p, b, t, first_slot(p, b))) * D + d0;
+    const Rotation rotation(load8<D>(p.q_weight + d0), load8<D>(p.cos + phase), load8<D>(p.sin + phase));
     auto finish = [&](float (&x)[kE], int h) {
-      norm_rope_fp32<D>(x, gain, p.q_eps, cos, sin, lane);
+      norm_rope_fp32<D>(x, p.q_eps, rotation);
       if (h >= heads) return;
       __nv_bfloat16* dst = out + static_cast<size_t>(h) * D;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
@@ -233,12 +260,7 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
         finish(x, h);
       }
     } else {
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.packed) + in;
-      for (int h0 = 0; h0 < heads; h0 += kMost * kRows) {
-        uint4 raw[kMost];
-#pragma unroll
-        for (int i = 0; i < kMost; ++i)
-          raw[i] = load8<D>(src + static_cast<size_t>(min(h0 + i * kRows + sub, heads - 1)) * D);
+      for (int h0 = 0;;) {
 #pragma unroll
         for (int i = 0; i < kMost; ++i) {
           if (h0 + i * kRows >= heads) break;  // warp-uniform
@@ -246,16 +268,18 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
           unpack8(raw[i], x);
           finish(x, h0 + i * kRows + sub);
         }
+        h0 += kMost * kRows;
+        if (h0 >= heads) break;
+        load(h0);
       }
     }
     return;
   }
-  if (kPart == kQueries) return;
 
   // ---- one cache block of one (row, KV head, K or V) ----
   __shared__ uint32_t s_largest[kWarps];
   __shared__ float s_finite[kWarps];
-  int item = blockIdx.x - (kPart == kBlocks ? 0 : p.query_ctas);
+  int item = block_cta;
   const int nth = item % p.touched;
   item /= p.touched;
   const bool is_value = item & 1;
@@ -274,9 +298,9 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
   const bool joins = start > low;  // the block holds earlier slots
   const float before = joins ? *scale_at : 0.f;
 
-  // this lane's slots of the block: warp * kRows + sub, and every kWarps * kRows from there
+  // this lane's slots of the block: warp * kRows + sub, and every kStride from there
   const int head = p.q_heads + (is_value ? p.kv_heads : 0) + h;
-  constexpr int kStep = kWarps * kRows, kSlots = kMaxBlock / kStep;
+  constexpr int kStride = kWarps * kRows, kSlots = kMaxBlock / kStride;
   const int slot0 = warp * kRows + sub;
   // slots that get a token
   const int from = static_cast<int>(start > low ? start - low : 0);
@@ -286,31 +310,44 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
     last = p.capacity - low;
   }
   const int to = static_cast<int>(last < p.block ? last : p.block);
+  // Every load of the lane's slots is issued before one is used. Slots that get no token count as zeros: a
+  // warp skips those of a pass where it has none that does, else they read the nearest such slot's token.
+  auto passes = [&](int i) {
+    const int first = warp * kRows + i * kStride;
+    return first < to && first + kRows > from;
+  };
   float x[kSlots][kE];
-  uint4 cos[kSlots], sin[kSlots], gain;
+  uint4 raw[kSlots], cos[2], sin[2], gain;  // cos and sin of two slots at a time: registers
+  auto token = [&](int i) { return static_cast<int>(low - start) + min(max(slot0 + i * kStride, from), to - 1); };
+  auto load_phase = [&](int i) {
+    if (is_value || !passes(i)) return;
+    const size_t phase = static_cast<size_t>(phase_row(p, b, token(i), start)) * D + d0;
+    cos[i & 1] = load8<D>(p.cos + phase);
+    sin[i & 1] = load8<D>(p.sin + phase);
+  };
   if (!is_value) gain = load8<D>(p.k_weight + d0);
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
-    const int slot = slot0 + i * kStep;
-    const bool fresh = slot >= from && slot < to;
-    if (fresh) {
-      const int t = static_cast<int>(low + slot - start);
-      load_packed8<D, kSplit>(p, (static_cast<size_t>(b) * p.tokens + t) * width + head * D + d0, split_stride, x[i]);
-      if (!is_value) {
-        const size_t phase = static_cast<size_t>(phase_row(p, b, t, start)) * D + d0;
-        cos[i] = load8<D>(p.cos + phase);
-        sin[i] = load8<D>(p.sin + phase);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) x[i][e] = 0.f;
-      cos[i] = sin[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (!passes(i)) continue;
+    const size_t off = (static_cast<size_t>(b) * p.tokens + token(i)) * width + head * D + d0;
+    if constexpr (kSplit)
+      load_packed8<D, true>(p, off, split_stride, x[i]);
+    else
+      raw[i] = load8<D>(static_cast<const __nv_bfloat16*>(p.packed) + off);
   }
+#pragma unroll
+  for (int i = 0; i < 2 && i < kSlots; ++i) load_phase(i);
   uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
-    if (!is_value) norm_rope_fp32<D>(x[i], gain, p.k_eps, cos[i], sin[i], lane);  // zeros stay zeros
+    const int slot = slot0 + i * kStride;
+    if (!kSplit) unpack8(raw[i], x[i]);
+    if (slot < from || slot >= to)
+#pragma unroll
+      for (int e = 0; e < kE; ++e) x[i][e] = 0.f;
+    if (!is_value && passes(i)) norm_rope_fp32<D>(x[i], p.k_eps, Rotation(gain, cos[i & 1], sin[i & 1]));  // zeros stay
+    if (i + 2 < kSlots) load_phase(i + 2);
     bits = max_bits(x[i], bits);
   }
   bits = __reduce_max_sync(0xffffffffu, bits);
@@ -334,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
   const float inverse = 1.f / after;
   if (joins && after > before) {
     const float ratio = before * inverse;
-    for (int slot = slot0; slot < from; slot += kStep) {
+    for (int slot = slot0; slot < from; slot += kStride) {
       float old[kE];
       load_codes8<D>(codes + static_cast<size_t>(slot) * D, old);
       store_codes8<D, true>(codes + static_cast<size_t>(slot) * D, old, ratio);
@@ -342,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, kSplit || kPart == kBoth ? 2 : kPart
   }
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
-    const int slot = slot0 + i * kStep;
+    const int slot = slot0 + i * kStride;
     if (slot < from || slot >= to) continue;
     if (sound)
       store_codes8<D, false>(codes + static_cast<size_t>(slot) * D, x[i], inverse);
@@ -403,17 +440,12 @@ __global__ void __launch_bounds__(128) relocate_kernel(uint8_t* store, float* sc
   if (lane == 0) s[to_block] = after;
 }
 
-constexpr long long kPromptRows = 1024;  // tokens from which Q heads and blocks take a launch each
+constexpr long long kPromptRows = 1024;
 
 template <int D, bool kSplit>
 int launch_append(const AppendParams& p, long long rows, long long ctas, cudaStream_t s) {
-  const dim3 threads(kThreads);
-  if (rows < kPromptRows)
-    return launch_ex(append_kernel<D, kSplit, kBoth>, dim3(static_cast<unsigned>(ctas)), threads, 0, s, 1, p);
-  const int st = launch_ex(append_kernel<D, kSplit, kQueries>, dim3(p.query_ctas), threads, 0, s, 1, p);
-  if (st != FB_OK) return st;
-  return launch_ex(append_kernel<D, kSplit, kBlocks>, dim3(static_cast<unsigned>(ctas - p.query_ctas)), threads, 0, s, 1,
-                   p);
+  auto* kernel = rows < kPromptRows ? append_kernel<D, kSplit, false> : append_kernel<D, kSplit, true>;
+  return launch_ex(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, s, 1, p);
 }
 
 }  // namespace q8

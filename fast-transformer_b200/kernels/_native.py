@@ -134,16 +134,23 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_current_device = torch._C._cuda_getDevice
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def launch(name, device, *args):
     """Calls entry point ``name`` with ``args`` and the current stream of ``device``, with that device
     current for the call (launch shapes and the error word go by the current device)."""
+    global launches
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        status = getattr(lib, name)(*args, _current_raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    check(status, name)
+            status = getattr(lib, name)(*args, _current_raw_stream(index))
+    if status != FB_OK:
+        check(status, name)
+    launches += _KERNELS_PER_CALL.get(name, 1)
 
 
 def ptr(tensor):

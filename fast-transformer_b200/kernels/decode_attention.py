@@ -143,8 +143,9 @@ def decode_attention_q8(query, cache, position, scale):
     or [B]. A row at position -1 (or below) holds nothing and gives zeros."""
     batch, q_heads, tokens, dim = query.shape
     assert tokens == 1 and batch == cache.batch and dim == cache.dim and q_heads % cache.kv_heads == 0
-    assert position.shape == (1,) or position.shape == (batch,)
-    return _attend_q8(query, cache, position, 1 if position.shape[0] > 1 else 0, None, 1, q_heads,
+    rows = position.numel()
+    assert position.dim() == 1 and (rows == 1 or rows == batch)
+    return _attend_q8(query, cache, position, 1 if rows > 1 else 0, None, 1, q_heads,
                       (batch, 1, q_heads, dim), scale)
 
 
