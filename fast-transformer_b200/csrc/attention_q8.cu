@@ -31,6 +31,7 @@
 //    ragged rows balance. A run of tiles that covers its unit writes the output; others leave
 //    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
 //    calls share nothing.
+#include <atomic>
 #include <type_traits>
 
 #include "q8.cuh"
@@ -98,13 +99,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// x - y where y may be -inf (an empty running maximum): the pivot is then 0.
-__device__ __forceinline__ float pivot(float m) { return m == -INFINITY ? 0.f : m; }
+// The pivot of nothing: finite, so that 2^(x - pivot) needs no test.
+constexpr float kNone = -3.402823466e38f;
 
 // sum p vs v / sum p from the two pivots' sums; zeros where nothing is seen, or only zero values.
 __device__ __forceinline__ float finished(float O, float M, float m, float l) {
-  if (l == 0.f || (M == -INFINITY && l > 0.f)) return 0.f;
-  return O / l * exp2f(pivot(M) - pivot(m));
+  if (l == 0.f || (M == kNone && l > 0.f)) return 0.f;
+  return O / l * exp2f(M - m);
 }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile written by TMA with rows of D bytes:
@@ -122,9 +123,10 @@ struct Smem {
   static constexpr int kStages = D == 128 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 5 : 4);
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kScaleBytes = kStages * kScales * 4;
-  static constexpr int kQueryPitch = D * 2 + 32;  // f16 query rows, padded against bank conflicts
-  static constexpr int kQuery = NG == 1 ? 0 : NG * 8 * kQueryPitch;
-  // P^T as B fragments, [slice][group][lane], of two tiles in turn
+  // queries as B fragments, [group][32 dims][lane], then every column's score multiplier and token
+  static constexpr int kFragments = NG * 8 * D * 2;
+  static constexpr int kQuery = NG == 1 ? 0 : kFragments + NG * 8 * 8;
+  // P^T as B fragments, [slice pair][group][lane][slice], of two tiles in turn
   static constexpr int kWeights = NG == 1 ? 0 : 2 * kSlices * NG * 32 * 8;
   // one group: half the dims of every warp; more: the O of warps that share dims with others
   static constexpr int kRedO = NG == 1 ? 4 * D / 2 * 8 * 4 : kSlices * NG * 32 * 16 / 2 * (D == 64);
@@ -206,7 +208,7 @@ __device__ __forceinline__ void clear(State<D, NG>& a) {
     for (int k = 0; k < State<D, NG>::kDims; ++k) a.o[n][k][0] = a.o[n][k][1] = a.o[n][k][2] = a.o[n][k][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      a.m[n][e] = a.M[n][e] = -INFINITY;
+      a.m[n][e] = a.M[n][e] = kNone;
       a.l[n][e] = 0.f;
     }
   }
@@ -243,25 +245,29 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
     const int first = up / 2;
     const float f0 = __uint_as_float(static_cast<uint32_t>(127 + first) << 23);
     const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up - first) << 23);
-    uint8_t* mine = query + col * S::kQueryPitch;
+    uint32_t f[D / 16][2];
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      const uint32_t b0 = pack_f16x2(bf16_lo(w[k].x) * f0 * f1, bf16_hi(w[k].x) * f0 * f1);
-      const uint32_t b1 = pack_f16x2(bf16_lo(w[k].y) * f0 * f1, bf16_hi(w[k].y) * f0 * f1);
+      f[k][0] = pack_f16x2(bf16_lo(w[k].x) * f0 * f1, bf16_hi(w[k].x) * f0 * f1);
+      f[k][1] = pack_f16x2(bf16_lo(w[k].y) * f0 * f1, bf16_hi(w[k].y) * f0 * f1);
       if constexpr (NG == 1) {
-        a.q[k][0] = b0;
-        a.q[k][1] = b1;
-      } else {
-        *reinterpret_cast<uint2*>(mine + (k * 16 + 4 * c) * 2) = make_uint2(b0, b1);
+        a.q[k][0] = f[k][0];
+        a.q[k][1] = f[k][1];
       }
     }
     const float multiplier = p.scale_log2 / f0 / f1;  // of column g; this thread's scores are 2c and 2c + 1
     if constexpr (NG == 1) {
       a.qs[0][0] = __shfl_sync(0xffffffffu, multiplier, 8 * c);
       a.qs[0][1] = __shfl_sync(0xffffffffu, multiplier, 8 * c + 4);
-    } else if (c == 0) {
-      *reinterpret_cast<float*>(mine + D * 2) = multiplier;
-      *reinterpret_cast<int*>(mine + D * 2 + 4) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        reinterpret_cast<uint4*>(query)[(warp * (D / 32) + i) * 32 + lane] =
+            make_uint4(f[2 * i][0], f[2 * i][1], f[2 * i + 1][0], f[2 * i + 1][1]);
+      if (c == 0) {
+        reinterpret_cast<float*>(query + S::kFragments)[col] = multiplier;
+        reinterpret_cast<int*>(query + S::kFragments)[NG * 8 + col] = t;
+      }
     }
   }
   if constexpr (NG > 1) {
@@ -269,8 +275,7 @@ __device__ __forceinline__ void start_unit(State<D, NG>& a, const Params& p, uin
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        a.qs[n][e] = *reinterpret_cast<const float*>(query + (n * 8 + 2 * c + e) * S::kQueryPitch + D * 2);
+      for (int e = 0; e < 2; ++e) a.qs[n][e] = reinterpret_cast<const float*>(query + S::kFragments)[n * 8 + 2 * c + e];
   }
   clear<D, NG>(a);
 }
@@ -408,7 +413,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
         m = fmaxf(m, top);
         M = fmaxf(M, top + lv[x]);
       }
-      const float fl = ex2(a.m[0][e] - pivot(m)), fo = ex2(a.M[0][e] - pivot(M));
+      const float fl = ex2(a.m[0][e] - m), fo = ex2(a.M[0][e] - M);
       a.m[0][e] = m;
       a.M[0][e] = M;
       a.l[0][e] *= fl;
@@ -420,7 +425,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
     }
   }
   uint32_t pb[H][2];
-  const float m0 = pivot(a.m[0][0]), m1 = pivot(a.m[0][1]), M0 = pivot(a.M[0][0]), M1 = pivot(a.M[0][1]);
+  const float m0 = a.m[0][0], m1 = a.m[0][1], M0 = a.M[0][0], M1 = a.M[0][1];
 #pragma unroll
   for (int x = 0; x < H; ++x) {
     a.l[0][0] += ex2(s[x][0] - m0) + ex2(s[x][2] - m0);
@@ -475,16 +480,16 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
   const int g = lane >> 2, c = lane & 3;
   const int slice = first + warp * 16;
   const int clear = p.chain != nullptr ? position + 1 : len;  // slots that every member sees
-  auto token = [&](int col) { return *reinterpret_cast<const int*>(sm.query + col * S::kQueryPitch + D * 2 + 4); };
+  auto token = [&](int col) { return reinterpret_cast<const int*>(sm.query + S::kFragments)[NG * 8 + col]; };
   float s[NG][4];
 #pragma unroll
   for (int n = 0; n < NG; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-  float lv = 0.f;
+  float ks = 0.f, lv = 0.f;
   if (slice < len) {
     const int row = warp * 16 + (lane & 15), half = lane >> 4;
-    const uint8_t* query = sm.query + g * S::kQueryPitch + 8 * c;
+    const uint4* query = reinterpret_cast<const uint4*>(sm.query) + lane;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       uint32_t r[4], k0[4], k1[4];
@@ -495,43 +500,52 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
       q8::e4m3x4_to_f16x4(r[3], k1[1], k1[3]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const uint8_t* src = query + n * 8 * S::kQueryPitch + i * 64;
-        const uint2 b0 = *reinterpret_cast<const uint2*>(src), b1 = *reinterpret_cast<const uint2*>(src + 32);
-        mma_f16(s[n], k0[0], k0[1], k0[2], k0[3], b0.x, b0.y);
-        mma_f16(s[n], k1[0], k1[1], k1[2], k1[3], b1.x, b1.y);
+        const uint4 q = query[(n * (D / 32) + i) * 32];
+        mma_f16(s[n], k0[0], k0[1], k0[2], k0[3], q.x, q.y);
+        mma_f16(s[n], k1[0], k1[1], k1[2], k1[3], q.z, q.w);
       }
     }
-    const float ks = scales[warp];
+    ks = scales[warp];
     lv = log2_scale(scales[kSlices + warp]);
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] *= a.qs[n][e & 1] * ks;
   }
+  uint32_t hidden = 0;  // a bit per score
   if (slice + 16 > clear) {
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (!sees(slice + g + (e >> 1) * 8, len, position, token(n * 8 + 2 * c + (e & 1)), chain)) s[n][e] = -INFINITY;
+        if (!sees(slice + g + (e >> 1) * 8, len, position, token(n * 8 + 2 * c + (e & 1)), chain)) hidden |= 1u << (n * 4 + e);
   }
-  bool moves = false;
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) moves = moves || fmaxf(s[n][e], s[n][e + 2]) > fminf(a.m[n][e], a.M[n][e] - lv) + kSlack;
-  uint2* weights = reinterpret_cast<uint2*>(sm.weights + k % 2 * (S::kWeights / 2)) + lane;
-  // weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile
-  for (;; fresh = moves = false) {
+  // The slice's weights, into this warp's half of its pair's fragments
+  uint2* weights =
+      reinterpret_cast<uint2*>(sm.weights + k % 2 * (S::kWeights / 2)) + warp / 2 * NG * 64 + lane * 2 + warp % 2;
+  float l[NG][2];
+  // Weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile.
+  for (;; fresh = false) {
     if (!fresh) {
+      float top = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const float f0 = lv - pivot(a.M[n][0]), f1 = lv - pivot(a.M[n][1]);
-        const uint32_t lo = movmatrix_trans(pack_f16x2(ex2(s[n][0] + f0), ex2(s[n][1] + f1)));
-        const uint32_t hi = movmatrix_trans(pack_f16x2(ex2(s[n][2] + f0), ex2(s[n][3] + f1)));
-        weights[(warp * NG + n) * 32] = make_uint2(lo, hi);
-    }
-      if (!consumers_any<NG>(moves)) break;
+        float x[4], y[4];  // s - m and s + log2 vs - M
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float by = a.qs[n][e & 1] * ks;
+          x[e] = fmaf(s[n][e], by, -a.m[n][e & 1]);
+          y[e] = fmaf(s[n][e], by, lv - a.M[n][e & 1]);
+        }
+        if (hidden != 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hidden >> (n * 4 + e) & 1) x[e] = y[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(x[e], y[e]));
+        weights[n * 64] = make_uint2(movmatrix_trans(pack_f16x2(ex2(y[0]), ex2(y[1]))),
+                                     movmatrix_trans(pack_f16x2(ex2(y[2]), ex2(y[3]))));
+        l[n][0] = ex2(x[0]) + ex2(x[2]);
+        l[n][1] = ex2(x[1]) + ex2(x[3]);
+      }
+      if (!consumers_any<NG>(top > kSlack)) break;
     }
     // [warp][column], where the last tile's weights were: everyone has multiplied by them (a run's first
     // tile: start_unit)
@@ -540,7 +554,9 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(s[n][e], s[n][e + 2]);
+        const float by = a.qs[n][e] * ks;
+        float top = fmaxf(hidden >> (n * 4 + e) & 1 ? -INFINITY : s[n][e] * by,
+                          hidden >> (n * 4 + e + 2) & 1 ? -INFINITY : s[n][e + 2] * by);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         if (g == 0) tops[warp * NG * 8 + n * 8 + 2 * c + e] = make_float2(top, top + lv);
@@ -560,7 +576,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
       for (int e = 0; e < 2; ++e) {
         const float m = fmaxf(a.m[n][e], __shfl_sync(0xffffffffu, top.x, n * 8 + 2 * c + e));
         const float M = fmaxf(a.M[n][e], __shfl_sync(0xffffffffu, top.y, n * 8 + 2 * c + e));
-        const float fl = ex2(a.m[n][e] - pivot(m)), fo = ex2(a.M[n][e] - pivot(M));
+        const float fl = ex2(a.m[n][e] - m), fo = ex2(a.M[n][e] - M);
         a.m[n][e] = m;
         a.M[n][e] = M;
         a.l[n][e] *= fl;
@@ -570,26 +586,25 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
   }
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
-    const float m0 = pivot(a.m[n][0]), m1 = pivot(a.m[n][1]);
-    a.l[n][0] += ex2(s[n][0] - m0) + ex2(s[n][2] - m0);
-    a.l[n][1] += ex2(s[n][1] - m1) + ex2(s[n][3] - m1);
+    a.l[n][0] += l[n][0];
+    a.l[n][1] += l[n][1];
   }
   constexpr int kChunks = D / 16, kShare = kSlices * kChunks / kConsumers<NG>;
   const int dims = warp % kChunks, from = warp / kChunks * kShare;
+  const uint4* pairs = reinterpret_cast<const uint4*>(sm.weights + k % 2 * (S::kWeights / 2)) + lane;
   if (first + kTile <= clear) {
 #pragma unroll
     for (int y0 = 0; y0 < kShare; y0 += 2) {
       uint32_t r[4];
       ldmatrix_x4_trans(vt + swizzled<D>(16 * (from + y0) + lane, dims), r[0], r[1], r[2], r[3]);
+      uint32_t f0[4], f1[4];
+      value_fragments(f0, r[0], r[1], kPick, kPick);
+      value_fragments(f1, r[2], r[3], kPick, kPick);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        uint32_t f[4];
-        value_fragments(f, r[2 * x], r[2 * x + 1], kPick, kPick);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          const uint2 pb = weights[((from + y0 + x) * NG + n) * 32];
-          mma_f16(a.o[n][0], f[0], f[1], f[2], f[3], pb.x, pb.y);
-        }
+      for (int n = 0; n < NG; ++n) {
+        const uint4 pb = pairs[((from + y0) / 2 * NG + n) * 32];
+        mma_f16(a.o[n][0], f0[0], f0[1], f0[2], f0[3], pb.x, pb.y);
+        mma_f16(a.o[n][0], f1[0], f1[1], f1[2], f1[3], pb.z, pb.w);
       }
     }
     return;
@@ -620,7 +635,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
 #pragma unroll
         for (int e = 0; e < 4; ++e) seen[e] = sees(at + 2 * c + (e & 1) + (e >> 1) * 8, len, position, t, chain);
         value_fragments(f, r[0], r[1], pick_slots(seen[0], seen[1]), pick_slots(seen[2], seen[3]));
-        const uint2 pb = weights[(y * NG + group) * 32];
+        const uint2 pb = reinterpret_cast<const uint2*>(pairs + (y / 2 * NG + group) * 32)[y % 2];
         float o[4] = {};
         mma_f16(o, f[0], f[1], f[2], f[3], pb.x, pb.y);
         if ((col & 7) >> 1 != c) continue;  // this thread's columns are 2c and 2c + 1
@@ -640,7 +655,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
                     pick_slots(2 * c + 8 < left, 2 * c + 9 < left));
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const uint2 pb = weights[(y * NG + n) * 32];
+      const uint2 pb = reinterpret_cast<const uint2*>(pairs + (y / 2 * NG + n) * 32)[y % 2];
       mma_f16(a.o[n][0], f[0], f[1], f[2], f[3], pb.x, pb.y);
     }
   }
@@ -682,7 +697,7 @@ __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& s
     for (int e0 = 0; e0 < 8 * (D / 2); e0 += kWarps * 32) {
       const int e = e0 + tid, col = e / (D / 2), d = e % (D / 2), in_chunk = n * 8 + col;
       if (in_chunk >= members) break;
-      float wM[kWarps], wm[kWarps], M = -INFINITY, m = -INFINITY;
+      float wM[kWarps], wm[kWarps], M = kNone, m = kNone;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* st = red_stats + (w * NG * 8 + in_chunk) * 3;
@@ -692,8 +707,8 @@ __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& s
       float O = 0.f, l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        O += red_o[(w * (D / 2) + d) * 8 + col] * ex2(wM[w] - pivot(M));
-        l += red_stats[(w * NG * 8 + in_chunk) * 3 + 2] * ex2(wm[w] - pivot(m));
+        O += red_o[(w * (D / 2) + d) * 8 + col] * ex2(wM[w] - M);
+        l += red_stats[(w * NG * 8 + in_chunk) * 3 + 2] * ex2(wm[w] - m);
       }
       sink(in_chunk, k0 * 16 + d, O, M, m, l);
     }
@@ -921,19 +936,19 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
     static_assert(kMaxCluster == 16, "a rank per lane of half a warp");
     const bool on = col < members && q < C;
     float* st = sm.recv_stats + (q * NG * 8 + col) * 3;
-    const float M_q = on ? st[0] : -INFINITY, m_q = on ? st[1] : -INFINITY;
+    const float M_q = on ? st[0] : kNone, m_q = on ? st[1] : kNone;
     float M = M_q, m = m_q;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) {
       M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     }
-    float l = on ? st[2] * ex2(m_q - pivot(m)) : 0.f;
+    float l = on ? st[2] * ex2(m_q - m) : 0.f;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     if (on) {
-      st[0] = ex2(M_q - pivot(M)) * finished(1.f, M, m, l);
-      st[2] = M == -INFINITY && l > 0.f ? 0.f : l;
+      st[0] = ex2(M_q - M) * finished(1.f, M, m, l);
+      st[2] = M == kNone && l > 0.f ? 0.f : l;
     }
   }
   consumers_sync<NG>();
@@ -1125,7 +1140,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   if (n > 0 && lo == hi) return;  // one run covered the unit and wrote its output
   for (int e = threadIdx.x; e < members * D; e += kMergeThreads) {
     const int col = col0 + e / D, d = e % D;
-    float M = -INFINITY, m = -INFINITY, O = 0.f, l = 0.f;
+    float M = kNone, m = kNone, O = 0.f, l = 0.f;
     if (n > 0) {
       const float4* st = p.stats + (static_cast<size_t>(lo) + blockIdx.x) * p.width + col;
       const float* acc = p.acc + ((static_cast<size_t>(lo) + blockIdx.x) * p.width + col) * D + d;
@@ -1138,7 +1153,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
           const int run = i0 + i;
           const bool on = run <= hi - lo &&
                           !(sparse && slice_start(T, lo + run, p.ctas) == slice_start(T, lo + run + 1, p.ctas));
-          s[i] = on ? __ldcg(st + static_cast<size_t>(run) * p.width) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+          s[i] = on ? __ldcg(st + static_cast<size_t>(run) * p.width) : make_float4(kNone, kNone, 0.f, 0.f);
           v[i] = on ? __ldcg(acc + static_cast<size_t>(run) * p.width * D) : 0.f;
         }
 #pragma unroll
@@ -1146,14 +1161,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
           tM = fmaxf(tM, s[i].x);
           tm = fmaxf(tm, s[i].y);
         }
-        O *= ex2(M - pivot(tM));
-        l *= ex2(m - pivot(tm));
+        O *= ex2(M - tM);
+        l *= ex2(m - tm);
         M = tM;
         m = tm;
 #pragma unroll
         for (int i = 0; i < kMergeRuns; ++i) {
-          O += v[i] * ex2(s[i].x - pivot(M));
-          l += s[i].z * ex2(s[i].y - pivot(m));
+          O += v[i] * ex2(s[i].x - M);
+          l += s[i].z * ex2(s[i].y - m);
         }
       }
     }
@@ -1206,7 +1221,7 @@ constexpr int kMaxDevices = 64;
 
 template <int D, int NG>
 bool configure() {
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   if (dev < kMaxDevices && configured[dev]) return true;
@@ -1223,7 +1238,7 @@ bool configure() {
 // Clusters of c CTAs that the device holds at once (0 if unknown), kept per device.
 template <int D, int NG>
 int resident_clusters(int c) {
-  static int cache[kMaxDevices][kMaxCluster + 1] = {};  // count + 1; 0: not asked
+  static std::atomic<int> cache[kMaxDevices][kMaxCluster + 1];  // count + 1; 0: not asked
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < kMaxDevices && cache[dev][c] != 0) return cache[dev][c] - 1;
