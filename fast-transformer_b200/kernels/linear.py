@@ -13,8 +13,8 @@ stay on cuBLAS through ``F.linear``, exactly as the reference routes them (linea
 search), so it only records the request.
 
 ``linear``, ``swiglu_linear`` and ``project`` also take 4-bit weights (kernels.quant.Weight4):
-fb_linear_w4 up to MAX_ROWS rows, one launch whose result is finished (never a ``Split``); more
-rows go to cuBLAS on the weights expanded to BF16 for the call. The reference has no such form.
+fb_linear_w4 for every MAX_ROWS rows up to MAX_ROWS4, one launch each whose result is finished (never a
+``Split``); more rows go to cuBLAS on the weights expanded to BF16 for the call. The reference has no such form.
 """
 
 import torch
@@ -27,6 +27,10 @@ from kernels.quant import Weight4
 
 #: Rows the skinny kernel takes (x is staged as 16/32/64-row slabs).
 MAX_ROWS = 64
+#: Rows that 4-bit weights take in launches of MAX_ROWS. 128 rows of [4096, 4096] in two: 17.9 us, expanded
+#: weights and cuBLAS 21.3 ([24576, 4096]: 71 and 125; [4096, 1024] loses 4 us); three launches of 192
+#: rows: 26.8 and 21.9.
+MAX_ROWS4 = 2 * MAX_ROWS
 BF16_OUT, FP32_OUT, SWIGLU_OUT, SPLITS_OUT = 0, 1, 2, 3
 _SPLITS = {}
 
@@ -78,26 +82,30 @@ def project(flat, weight, epilogue=BF16_OUT, splits=None):
 
 
 def _launch4(x, weight, out, rows, epilogue):
-    """fb_linear_w4 on contiguous x of ``rows`` rows."""
+    """fb_linear_w4 on contiguous x of ``rows`` rows, MAX_ROWS of them at a time."""
     device = weight.device
     if x.device != device:
         raise ValueError(f"4-bit weights on {device} take inputs of that device, not {x.device}")
     if x.data_ptr() % 16:
         x = x.clone()
-    launch("fb_linear_w4", device, x.data_ptr(), weight.packed.data_ptr(), out.data_ptr(), rows, weight.n, weight.k, weight.group,
-           epilogue)
+    source, target, packed = x.data_ptr(), out.data_ptr(), weight.packed.data_ptr()
+    n, k, group = weight.n, weight.k, weight.group
+    launch("fb_linear_w4", device, source, packed, target, min(rows, MAX_ROWS), n, k, group, epilogue)
+    for row in range(MAX_ROWS, rows, MAX_ROWS):
+        launch("fb_linear_w4", device, source + row * k * 2, packed, target + row * (out.nbytes // rows),
+               min(rows - row, MAX_ROWS), n, k, group, epilogue)
     return out
 
 
 def _refuse4(x, weight):
-    raise ValueError(f"4-bit weights {tuple(weight.shape)} take 1 to {MAX_ROWS} BF16 rows of their width, not {x.dtype} "
-                     f"{tuple(x.shape)}")
+    raise ValueError(f"4-bit weights {tuple(weight.shape)} take 1 to {MAX_ROWS4} BF16 rows of their width, not "
+                     f"{x.dtype} {tuple(x.shape)}")
 
 
 def _project4(flat, weight, epilogue):
     """fb_linear_w4 on [M,K]: the outputs of ``project``."""
     m, n = flat.shape[0], weight.n
-    if flat.shape[1] != weight.k or flat.dtype != torch.bfloat16 or not 0 < m <= MAX_ROWS:
+    if flat.shape[1] != weight.k or flat.dtype != torch.bfloat16 or not 0 < m <= MAX_ROWS4:
         _refuse4(flat, weight)
     if epilogue == SWIGLU_OUT:
         if n % 128:
@@ -115,7 +123,7 @@ def _linear4(x, weight):
     if shape[-1] != k or x.dtype != torch.bfloat16:
         _refuse4(x, weight)
     rows = x.numel() // k
-    if rows > MAX_ROWS:
+    if rows > MAX_ROWS4:
         _native.require_device(weight.device, x)
         return F.linear(x, weight.dequantized())
     out = x.new_empty(*shape[:-1], weight.n)

@@ -216,6 +216,76 @@ def test_block_attention_hides_nan_of_later_drafts(dim):
     assert ((out.double() - expect).abs()[hidden] <= bound[hidden]).all()
 
 
+@pytest.mark.parametrize("tokens,dim", [(3, 64), (3, 128), (5, 64), (5, 128), (8, 64), (8, 128), (1, 128)])
+def test_block_attention_many_ragged_rows(tokens, dim):
+    """More units than SMs (slices of a persistent grid that split units and cross them), two to four column
+    groups, rows from empty to several tiles."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(100 * tokens + dim)
+    batch, capacity = 20, 700
+    position = torch.randint(-1, capacity - tokens + 1, (batch,), generator=g)
+    position[:4] = torch.tensor([-1, 0, capacity - tokens, 127])
+    chain = torch.randint(1, tokens + 1, (batch,), generator=g)
+    cache = oq.random_cache(batch, 8, capacity, dim, 32, g)
+    poison(cache, position, tokens)
+    query = torch.randn(batch, tokens, 32, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, cache, position, 1 / math.sqrt(dim), chain)
+    out = block_attention_q8(query.to(DEV), handle(cache), position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV))
+    check_attention(out, expect, bound)
+    assert (out[0] == 0).all()
+
+
+@pytest.mark.parametrize("batch", [2, 40])
+@pytest.mark.parametrize("tokens,dim", [(1, 128), (3, 128), (5, 64), (7, 128)])
+def test_block_attention_rising_scores_and_uneven_scales(batch, tokens, dim):
+    """Scores that rise from block to block, so that the pivots move in every tile, and value scales 2^40
+    apart, 2^-100 or 0, so that the value product's pivot moves on its own."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(batch + tokens)
+    capacity, kv_heads = 800, 4
+    cache = oq.random_cache(batch, kv_heads, capacity, dim, 64, g)
+    blocks = cache["key_scales"].shape[2]
+    cache["key_scales"] *= torch.exp2(torch.linspace(-2, 3, blocks).round())
+    cache["value_scales"][0] = torch.exp2(torch.linspace(-30, 10, blocks).round())
+    cache["value_scales"][1] = torch.exp2(torch.linspace(10, -30, blocks).round())
+    cache["value_scales"][1, :, ::3] = 0.0
+    if batch > 2:
+        cache["value_scales"][2] = 0.0
+        cache["values"][3] = torch.zeros(kv_heads, capacity, dim).to(oq.E4M3)
+        cache["value_scales"][3] = 2.0 ** -100
+        cache["value_scales"][4] *= 1.37
+        cache["key_scales"][4] *= 0.81
+    position = torch.full((batch,), capacity - tokens)
+    chain = torch.full((batch,), tokens)
+    query = torch.randn(batch, tokens, kv_heads * 4, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, cache, position, 1 / math.sqrt(dim), chain)
+    out = block_attention_q8(query.to(DEV), handle(cache), position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV))
+    check_attention(out, expect, bound + 1e-40)
+
+
+@pytest.mark.parametrize("tokens,dim", [(2, 128), (4, 64), (4, 128), (8, 128)])
+def test_block_attention_hides_nan_in_many_rows(tokens, dim):
+    """The same where slices of the grid end inside the rows, with the NaN in the last draft's slot."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(tokens + dim)
+    batch, capacity = 24, 300
+    position = torch.randint(0, capacity - tokens + 1, (batch,), generator=g)
+    chain = torch.full((batch,), tokens)
+    cache = oq.random_cache(batch, 8, capacity, dim, 16, g)
+    poison(cache, position, tokens)
+    sound = {k: v.clone() if torch.is_tensor(v) else v for k, v in cache.items()}
+    for b in range(batch):
+        cache["values"].view(torch.uint8)[b, :, int(position[b]) + tokens - 1, 9] = 0xff
+    query = torch.randn(batch, tokens, 32, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, sound, position, 0.1, chain)
+    out = block_attention_q8(query.to(DEV), handle(cache), position.to(DEV), 0.1, chain.to(DEV)).cpu()
+    assert torch.isnan(out[:, -1, :, 9]).all()
+    hidden = torch.ones_like(out, dtype=torch.bool)
+    hidden[:, -1, :, 9] = False
+    assert torch.isfinite(out[hidden]).all()
+    assert ((out.double() - expect).abs()[hidden] <= bound[hidden]).all()
+
+
 # ------------------------------------------------------------------------------ append
 def append_case(batch, tokens, q_heads, kv_heads, dim, capacity, block, mode, starts, seed):
     g = torch.Generator().manual_seed(seed)
@@ -507,3 +577,60 @@ def test_quantize_weight4_is_nearest():
     off = (w.view(48, 4, 64) - parts).abs()
     assert (off <= (0.5 + 7 * 2.0 ** -8) * step[..., None] + 2.0 ** -8 * parts.abs() + 1e-12).all()
     assert (w.view(48, 4, 64)[3, 1] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [65, 100, 128, 129, 300])
+def test_linear_more_rows_than_a_launch_takes(rows):
+    """Two launches up to 128 rows, expanded weights above (rounded once to bf16: 2^-8 of each product)."""
+    from kernels import linear as klinear
+    from kernels.quant import pack_weight4
+    codes, scales, g = weights(256, 320, 64, rows)
+    w = pack_weight4(codes.to(DEV), scales.to(DEV))
+    x = torch.randn(rows, 320, generator=g).bfloat16()
+    y, size = oq.linear(x, codes, scales)
+    expanded = 0.0 if rows <= 128 else 2.0 ** -8
+    assert ((klinear.linear(x.to(DEV), w).cpu().double() - y).abs() <= oq.linear_bound(y, size, 320) + expanded * size).all()
+    if rows > 128:
+        with pytest.raises(ValueError):
+            klinear.swiglu_linear(x.to(DEV), w)
+        return
+    for epilogue in (klinear.BF16_OUT, klinear.FP32_OUT, klinear.SPLITS_OUT, klinear.SWIGLU_OUT):
+        whole = klinear.project(x.to(DEV), w, epilogue)
+        parts = [klinear.project(x[a:b].contiguous().to(DEV), w, epilogue) for a, b in ((0, 64), (64, rows))]
+        assert torch.equal(whole, torch.cat(parts, 1 if epilogue == klinear.SPLITS_OUT else 0))
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap on the GPU share nothing: the results are those of calls in turn."""
+    from kernels.decode_attention import block_attention_q8, decode_attention_q8
+    from kernels.linear import linear
+    from kernels.quant import quantize_weight4
+    g = torch.Generator().manual_seed(31)
+    jobs = []
+    for i in range(2):
+        small, large = (handle(oq.random_cache(b, 8, 600, 128, 64, g)) for b in (2, 24))
+        w = quantize_weight4(torch.randn(2048, 1024, generator=g).bfloat16().to(DEV), 64)
+        x = torch.randn(7 + i, 1024, generator=g).bfloat16().to(DEV)
+        q = torch.randn(24, 5, 32, 128, generator=g).bfloat16().to(DEV)
+        first = torch.randint(0, 595, (24,), generator=g).to(DEV)
+        chain = torch.full((24,), 5).to(DEV)
+
+        def job(small=small, large=large, w=w, x=x, q=q, first=first, chain=chain):
+            one = q[:, :1].transpose(1, 2).contiguous()
+            return (linear(x, w), decode_attention_q8(one[:2], small, first[:2], 0.09),
+                    block_attention_q8(q[:2].contiguous(), small, first[:2], 0.09, chain[:2]),
+                    decode_attention_q8(one, large, first, 0.09), block_attention_q8(q, large, first, 0.09, chain))
+
+        jobs.append(job)
+    expect = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], [[], []]
+    for _ in range(10):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(job())
+    torch.cuda.synchronize()
+    for want, runs in zip(expect, got):
+        for run in runs:
+            for a, b in zip(want, run):
+                assert torch.equal(a, b)
