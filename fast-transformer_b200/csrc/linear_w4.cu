@@ -146,7 +146,11 @@ struct Config {
   static constexpr int kFree = (228 * 1024) / kCtas - 1024 - 1024 - kRecv - 256;
   static constexpr int NS = kFree / kStage > 8 ? 8 : kFree / kStage;
   static constexpr int kTotal = 1024 + NS * kStage + kRecv + 256;
-  static_assert(NS >= 2 && kTotal <= 227 * 1024, "shared memory");
+  static_assert(kTotal <= 227 * 1024, "shared memory");
+  // An odd number of stages gives a stage to the two sets in turn, so a set sees every other phase of its
+  // barrier and must not come back before the other's use has landed. The MMA warp takes parts in order:
+  // while part u is missing a set waits for at most part u + 3.
+  static_assert(NS >= 4 && kSets == 2, "a stage's next use lies beyond a set's lead");
 };
 
 template <typename C>
