@@ -25,9 +25,9 @@
 //    would not fit the registers. Eight consumers: each scores its slice, P^T goes to shared memory, and
 //    each multiplies all of it by its 16 dims of V. One barrier a tile (the vote), O held once.
 // Work is cut in one of two ways:
-//  * Few units: a cluster of C CTAs per unit (interleaved tiles), merged by pushing each
+//  * Few units, or short rows: a cluster of C CTAs per unit (interleaved tiles), merged by pushing each
 //    partial to its output's owner through distributed shared memory: one launch, no workspace.
-//  * Many units: a persistent grid cuts the tiles of all units into equal contiguous slices, so
+//  * Many units of long rows: a persistent grid cuts the tiles of all units into equal contiguous slices, so
 //    ragged rows balance. A run of tiles that covers its unit writes the output; others leave
 //    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
 //    calls share nothing.
@@ -1262,13 +1262,19 @@ int resident_clusters(int c) {
   return n;
 }
 
-// The cluster size of a launch, 0 for the persistent form: the largest whose clusters are all
-// resident at once, no larger than the cache has tiles.
+// Tiles up to which a CTA per unit beats the persistent form's slices whatever the lengths: the merge and the
+// partials cost more than uneven rows. 64 rows of 8 KV heads: up to 4101 slots of any length 59 us against 92,
+// 4101 slots each 86 against 92; 24 rows of up to 8197 slots 58 against 47, of up to 32768 240 against 156.
+constexpr int kUnitTiles = 36;
+
+// The cluster size of a launch, 0 for the persistent form. Up to a unit per SM: the largest whose clusters are
+// all resident at once, no larger than the cache has tiles (64 units of 33 tiles, 20 members: 28 us, the
+// persistent form 43).
 template <int D, int NG>
 int cluster_size(const Params& p) {
-  const int units = p.batch * p.kv_heads * p.chunks;
-  if (units > sm_count() || units > 65535) return 0;
-  const int tiles = tiles_of(p.capacity);
+  const int units = p.batch * p.kv_heads * p.chunks, tiles = tiles_of(p.capacity);
+  if (units > 65535) return 0;
+  if (units > sm_count()) return tiles <= kUnitTiles ? 1 : 0;
   for (int c = tiles < kMaxCluster ? tiles : kMaxCluster; c >= 1; --c)
     if (resident_clusters<D, NG>(c) >= units) return c;
   return 0;

@@ -235,6 +235,31 @@ def test_block_attention_many_ragged_rows(tokens, dim):
     assert (out[0] == 0).all()
 
 
+@pytest.mark.parametrize("tokens,dim,q_heads", [(1, 64, 8), (2, 64, 48), (3, 128, 56), (4, 64, 64)])
+def test_block_attention_slices_of_long_rows(tokens, dim, q_heads):
+    """A capacity from which many units are cut into slices: a few long rows among short ones, one to four
+    column groups, a NaN in one row's last draft."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(tokens * dim)
+    batch, capacity, kv_heads = 19, 4800, 8
+    position = torch.randint(-1, 400, (batch,), generator=g)
+    position[3], position[4], position[11] = capacity - tokens, -1, 2000
+    chain = torch.randint(1, tokens + 1, (batch,), generator=g)
+    cache = oq.random_cache(batch, kv_heads, capacity, dim, 64, g)
+    poison(cache, position, tokens)
+    sound = {k: v.clone() if torch.is_tensor(v) else v for k, v in cache.items()}
+    cache["values"].view(torch.uint8)[11, :, 2000 + tokens - 1, 9] = 0xff
+    chain[11] = tokens
+    query = torch.randn(batch, tokens, q_heads, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, sound, position, 1 / math.sqrt(dim), chain)
+    out = block_attention_q8(query.to(DEV), handle(cache), position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV)).cpu()
+    assert torch.isnan(out[11, -1, :, 9]).all() and (out[4] == 0).all()
+    kept = torch.ones_like(out, dtype=torch.bool)
+    kept[11, -1, :, 9] = False
+    assert torch.isfinite(out[kept]).all()
+    assert ((out.double() - expect).abs()[kept] <= bound[kept]).all()
+
+
 @pytest.mark.parametrize("batch", [2, 40])
 @pytest.mark.parametrize("tokens,dim", [(1, 128), (3, 128), (5, 64), (7, 128)])
 def test_block_attention_rising_scores_and_uneven_scales(batch, tokens, dim):
