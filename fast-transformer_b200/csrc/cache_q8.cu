@@ -15,10 +15,14 @@
 // largest magnitude through shared memory, and is the only reader and writer of the block's
 // codes and scale. No atomics. Q heads run in CTAs of their own, a warp per token and run of heads.
 //
-// A prompt is bound by bytes (the packed projection in, Q and the codes out) and close behind by
-// instructions: a head's D values lie on D / 8 lanes, four dims of each half, so that RoPE's partners
-// meet in a lane (no shuffles but the norm's), and a warp issues all the loads of its rows before it
-// uses one. A decode step is bound by latency.
+// A prompt is bound by instruction issue (0.75 per cycle) and close behind by bytes (the packed projection
+// in, Q and the codes out): a head's D values lie on D / 8 lanes, four dims of each half, so that RoPE's
+// partners meet in a lane (no shuffles but the norm's); gains are folded into cos and sin once per token; the
+// arithmetic runs in fp32 pairs; and a warp issues all the loads of its rows before it uses one. 8192 tokens of
+// 32 + 8 heads of 128: 36.9 us, 5.1 TB/s, 0.78 of the floor. (Of the steps: loads that waited for one another
+// 55 us; a launch each for Q heads and blocks 50; all cos and sin loaded at once, three CTAs per SM, 49;
+// gains, cos and sin applied one by one, and single fp32 operations, 43; eight heads a warp instead of sixteen 39.)
+// A decode step is bound by latency: 16 rows 2.9 us.
 #include <initializer_list>
 
 #include "q8.cuh"
@@ -122,19 +126,38 @@ __device__ __forceinline__ void load_packed8(const AppendParams& p, size_t off, 
   for (int e = 0; e < kE; ++e) x[e] = bf16_round(x[e]);
 }
 
-// gain * cos and the partner's gain * sin of a lane's dims: RoPE of x * inv * gain is then
-// inv * (x c -+ partner s).
+// Two fp32 operations in one instruction (sm_100): a prompt is bound by issue.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; "
+      "fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+// gain * cos and the partner's -+ gain * sin of a lane's dims, in pairs: RoPE of x * inv * gain is then
+// inv * (x c + partner s).
 struct Rotation {
-  float c[kE], s[kE];
+  float2 c[kE / 2], s[kE / 2];
   __device__ __forceinline__ Rotation(const uint4& gain, const uint4& cos, const uint4& sin) {
-    float g[kE];
+    float g[kE], cs[kE], sn[kE];
     unpack8(gain, g);
-    unpack8(cos, c);
-    unpack8(sin, s);
+    unpack8(cos, cs);
+    unpack8(sin, sn);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      c[e] *= g[e];
-      s[e] *= g[e ^ 4];
+    for (int i = 0; i < kE / 2; ++i) {
+      const int e = 2 * i;
+      const float sign = i < kE / 4 ? -1.f : 1.f;
+      c[i] = make_float2(g[e] * cs[e], g[e + 1] * cs[e + 1]);
+      s[i] = make_float2(sign * g[e ^ 4] * sn[e], sign * g[(e + 1) ^ 4] * sn[e + 1]);
     }
   }
 };
@@ -143,17 +166,23 @@ struct Rotation {
 template <int D>
 __device__ __forceinline__ void norm_rope_fp32(float (&x)[kE], float eps, const Rotation& r) {
   constexpr int kLanes = Lanes<D>::kLanes;
-  float ss = 0.f;
+  float2 v[kE / 2], sum = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int e = 0; e < kE; ++e) ss += x[e] * x[e];
+  for (int i = 0; i < kE / 2; ++i) {
+    v[i] = make_float2(x[2 * i], x[2 * i + 1]);
+    sum = fma2(v[i], v[i], sum);
+  }
+  float ss = sum.x + sum.y;
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float inv = __frsqrt_rn(ss / static_cast<float>(D) + eps);
+  const float inv = rsqrtf(ss / static_cast<float>(D) + eps);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float low = x[e] * inv, high = x[e + 4] * inv;
-    x[e] = low * r.c[e] - high * r.s[e];
-    x[e + 4] = high * r.c[e + 4] + low * r.s[e + 4];
+  for (int i = 0; i < kE / 2; ++i) v[i] = mul2(v[i], make_float2(inv, inv));
+#pragma unroll
+  for (int i = 0; i < kE / 2; ++i) {
+    const float2 out = fma2(v[i ^ 2], r.s[i], mul2(v[i], r.c[i]));
+    x[2 * i] = out.x;
+    x[2 * i + 1] = out.y;
   }
 }
 
@@ -185,10 +214,11 @@ __device__ __forceinline__ void load_codes8(const uint8_t* src, float (&x)[kE]) 
 
 constexpr uint32_t kInfinity = 0x7f800000u;  // bits: anything from here on is not finite
 
-// Bits of the largest magnitude (they order as the magnitudes do; NaN above infinity above all).
-__device__ __forceinline__ uint32_t max_bits(const float (&x)[kE], uint32_t so_far) {
+// The largest magnitude, or NaN (its bits order as magnitudes do; NaN above infinity above all).
+__device__ __forceinline__ float largest_magnitude(const float (&x)[kE], float so_far) {
 #pragma unroll
-  for (int e = 0; e < kE; ++e) so_far = max(so_far, __float_as_uint(x[e]) & 0x7fffffffu);
+  for (int e = 0; e < kE; e += 2)
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(so_far) : "f"(fabsf(x[e])), "f"(fabsf(x[e + 1])));
   return so_far;
 }
 
@@ -203,9 +233,7 @@ __device__ __forceinline__ float finite_max(const float (&x)[kE], float so_far) 
 }
 
 // One launch does both. A decode step's CTAs of Q heads come first; a prompt's CTAs of either kind are spread
-// evenly, so that the blocks' chains of loads, norm, barrier and stores hide behind the Q heads' bytes
-// (8192 tokens of 32 + 8 heads of 128: 42.7 us, 4.4 TB/s; a launch of each kind 50.3; 48.9 with all cos and
-// sin loaded at once, three CTAs per SM instead of four).
+// evenly, so that the blocks' chains of loads, norm, barrier and stores hide behind the Q heads' bytes.
 template <int D, bool kSplit, bool kPrompt>
 __global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_kernel(const AppendParams p) {
   constexpr int kLanes = Lanes<D>::kLanes, kRows = Lanes<D>::kRows;
@@ -338,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_k
   }
 #pragma unroll
   for (int i = 0; i < 2 && i < kSlots; ++i) load_phase(i);
-  uint32_t bits = 0;
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     const int slot = slot0 + i * kStride;
@@ -348,9 +376,9 @@ __global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_k
       for (int e = 0; e < kE; ++e) x[i][e] = 0.f;
     if (!is_value && passes(i)) norm_rope_fp32<D>(x[i], p.k_eps, Rotation(gain, cos[i & 1], sin[i & 1]));  // zeros stay
     if (i + 2 < kSlots) load_phase(i + 2);
-    bits = max_bits(x[i], bits);
+    top = largest_magnitude(x[i], top);
   }
-  bits = __reduce_max_sync(0xffffffffu, bits);
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if (lane == 0) s_largest[warp] = bits;
   __syncthreads();
 #pragma unroll
@@ -499,10 +527,10 @@ extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, 
   p.err = error_word();
   // a prompt starts on a block; elsewhere the first token can be a block's last slot
   p.touched = mode == 1 ? (tokens + block - 1) / block : (tokens + block - 2) / block + 1;
-  // a prompt's warps take eight heads of a token (four loads in flight at D = 128), a few rows' the least
-  // that fills a load, so that more warps share them
+  // a prompt's warps take sixteen heads of a token (its rotation is worked out once for them), a few rows' the
+  // least that fills a load, so that more warps share them
   const long long rows = static_cast<long long>(batch) * tokens;
-  p.query_heads = rows >= q8::kPromptRows ? 8 : 32 * q8::kE / head_dim;
+  p.query_heads = rows >= q8::kPromptRows ? 16 : 32 * q8::kE / head_dim;
   p.runs = (q_heads + p.query_heads - 1) / p.query_heads;
   const long long query_ctas = (rows * p.runs + q8::kWarps - 1) / q8::kWarps;
   const long long ctas = query_ctas + 2ll * batch * kv_heads * p.touched;
