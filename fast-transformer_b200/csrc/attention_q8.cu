@@ -9,9 +9,10 @@
 // The codes are never expanded in memory: a warp converts its e4m3 fragments to f16 (exact) on
 // the way into mma.sync m16n8k16, and the scales, uniform over a warp's 16 slots, fold into
 // scalars. K's multiplies the scores. V's joins the exponent: the value product takes
-// p'[c] = 2^(s[c] + log2 vs - M) with a pivot M of its own over s + log2 vs, so a block's scale
+// p'[c] = 2^(s[c] - m + log2 vs - r) with a pivot r of its own over s - m + log2 vs, so a block's scale
 // can neither overflow nor wash out P's f16 range, while the denominator sums 2^(s - m) in
-// fp32. Q is scaled by a power of two to f16's range (exact for any bf16 row).
+// fp32. r is kept relative to m: where scores are so large that their own rounding passes 1, the result is
+// still a mean of values. Q is scaled by a power of two to f16's range (exact for any bf16 row).
 //
 // Bound by the bytes of codes. Members = the T * G query heads that share a KV head, in groups of
 // 8 NG columns; a unit = (row, KV head, member group); its tiles are 128 slots of K and V. A CTA is
@@ -31,6 +32,10 @@
 //    ragged rows balance. A run of tiles that covers its unit writes the output; others leave
 //    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
 //    calls share nothing.
+// Measured (D = 128, blocks of 64): 16 rows x 8320 slots, 32 + 8 heads 45.4 us, 6.0 TB/s (0.92 of a copy's rate);
+// 64 rows of 1024 to 32768 slots 349 us, 6.3 TB/s; one row of 2048 slots 5.6 us, most of it launch, the chain
+// position - tile - product, and the merge; 8 rows x 4101 slots x 5 tokens 28.5 us, 2.4 TB/s: 0.36 of the issue
+// slots, the warps waiting on each other's weights, on conversions and on shared memory.
 #include <atomic>
 #include <type_traits>
 
@@ -59,7 +64,7 @@ struct Params {
   int per_row;
   __nv_bfloat16* out;  // [B, T, Hq, D]
   float* acc;          // [ctas + units, width, D]
-  float4* stats;       // [ctas + units, width]: M, m, l
+  float4* stats;       // [ctas + units, width]: r, m, l
   int batch, tokens, q_heads, kv_heads, groups, capacity, block, blocks, ctas;
   int members;  // T * G
   int chunks;   // member groups per (row, KV head)
@@ -101,11 +106,13 @@ __device__ __forceinline__ float ex2(float x) {
 
 // The pivot of nothing: finite, so that 2^(x - pivot) needs no test.
 constexpr float kNone = -3.402823466e38f;
+// A pivot relative to one m, relative to another that lies `by` below.
+__device__ __forceinline__ float shifted(float r, float by) { return fmaxf(kNone, r + by); }
 
 // sum p vs v / sum p from the two pivots' sums; zeros where nothing is seen, or only zero values.
-__device__ __forceinline__ float finished(float O, float M, float m, float l) {
-  if (l == 0.f || (M == kNone && l > 0.f)) return 0.f;
-  return O / l * exp2f(M - m);
+__device__ __forceinline__ float finished(float O, float r, float l) {
+  if (l == 0.f || (r == kNone && l > 0.f)) return 0.f;
+  return O / l * exp2f(r);
 }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile written by TMA with rows of D bytes:
@@ -130,15 +137,16 @@ struct Smem {
   static constexpr int kWeights = NG == 1 ? 0 : 2 * kSlices * NG * 32 * 8;
   // one group: half the dims of every warp; more: the O of warps that share dims with others
   static constexpr int kRedO = NG == 1 ? 4 * D / 2 * 8 * 4 : kSlices * NG * 32 * 16 / 2 * (D == 64);
-  static constexpr int kRedStats = NG == 1 ? kConsumers<NG> * 8 * 3 * 4 : 0;  // M, m, l
+  static constexpr int kRedStats = NG == 1 ? kConsumers<NG> * 8 * 3 * 4 : 0;  // r, m, l
   // persistent form: tile counts before each row; cluster form: O received as an owner
-  // ([rank][chunk], C * 2 ceil(n / 2C) < n + 2C values) and every rank's M, m, l
+  // ([rank][chunk], C * 2 ceil(n / 2C) < n + 2C values) and every rank's r, m, l
   static constexpr int kCum = ((kMaxBatch + 1) * 4 + 15) & ~15;
   static constexpr int kRecvO = (NG * 8 * D + 2 * kMaxCluster) * 4;
   static constexpr int kRecvStats = kMaxCluster * NG * 8 * 3 * 4;
   static constexpr int kShared = kCum > kRecvO + kRecvStats ? kCum : kRecvO + kRecvStats;
   static constexpr int kBars = 2 * kStages * 8;
-  static constexpr int kTotal = 1024 + kRing + kScaleBytes + kQuery + kWeights + kRedO + kRedStats + kShared + kBars + 32;
+  static constexpr int kTotal =
+      1024 + kRing + kScaleBytes + kQuery + kWeights + kRedO + kRedStats + kShared + kBars + 64;
   static_assert(kTotal + 1024 <= 228 * 1024 / 2, "two CTAs per SM");
   static_assert((kScaleBytes + kQuery + kWeights + kRedO + kRedStats + kShared) % 16 == 0, "mbarrier alignment");
 
@@ -153,7 +161,7 @@ struct Smem {
   float* recv_stats;
   uint64_t* full;
   uint64_t* empty;
-  volatile int* misc;  // [0..2]: first row, unit, tile; [3]: abort
+  volatile int* misc;  // [0..2]: first row, unit, tile; [3]: abort; [4 + warp]: 1 + the tile of its last move
 
   __device__ explicit Smem(uint8_t* raw) {
     ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -179,7 +187,7 @@ struct State {
   static constexpr int kDims = NG == 1 ? D / 16 : 1;
   uint32_t q[NG == 1 ? D / 16 : 1][2];
   float o[NG][kDims][4];
-  float m[NG][2], M[NG][2], l[NG][2];  // columns 2c, 2c + 1
+  float m[NG][2], r[NG][2], l[NG][2];  // columns 2c, 2c + 1
   float qs[NG][2];                     // score multiplier of those columns: 2^e scale log2(e)
 };
 
@@ -208,7 +216,7 @@ __device__ __forceinline__ void clear(State<D, NG>& a) {
     for (int k = 0; k < State<D, NG>::kDims; ++k) a.o[n][k][0] = a.o[n][k][1] = a.o[n][k][2] = a.o[n][k][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      a.m[n][e] = a.M[n][e] = kNone;
+      a.m[n][e] = a.r[n][e] = kNone;
       a.l[n][e] = 0.f;
     }
   }
@@ -348,8 +356,8 @@ __device__ __forceinline__ float log2_scale(float x) {
 // `position`: its first token's slot; scales: the tile's, K then V.
 template <int D>
 __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, const Smem<D, 1>&, const float* scales,
-                                            uint32_t kt, uint32_t vt, int, bool, int first, int len, int position, int chain,
-                                            int chunk, int warp, int lane) {
+                                            uint32_t kt, uint32_t vt, int, bool, int first, int len, int position,
+                                            int chain, int chunk, int warp, int lane) {
   constexpr int H = 2;
   const int g = lane >> 2, c = lane & 3, half = lane >> 4;
   const int slice = first + warp * 32;
@@ -381,7 +389,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
     const float ks = live ? scales[warp * 2 + x] : 1.f;
     lv[x] = live ? log2_scale(scales[kSlices + warp * 2 + x]) : 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[x][e] = (s[x][e] + s2[x][e]) * (a.qs[0][e & 1] * ks);
+    for (int e = 0; e < 4; ++e) s[x][e] = __fmul_rn(s[x][e] + s2[x][e], a.qs[0][e & 1] * ks);
   }
   // every member sees slots [0, position]; past them the chain rule decides per token
   const bool tail = slice + 16 * H > (p.chain != nullptr ? position + 1 : len);
@@ -399,23 +407,28 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
 #pragma unroll
   for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int x = 0; x < H; ++x)
-      moves = moves || fmaxf(s[x][e], s[x][e + 2]) > fminf(a.m[0][e], a.M[0][e] - lv[x]) + kSlack;
+    for (int x = 0; x < H; ++x) {
+      const float over = fmaxf(s[x][e], s[x][e + 2]) - a.m[0][e];
+      moves = moves || fmaxf(over, over + lv[x] - a.r[0][e]) > kSlack;
+    }
   if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float m = a.m[0][e], M = a.M[0][e];
+      float top[H], m = a.m[0][e];
 #pragma unroll
       for (int x = 0; x < H; ++x) {
-        float top = fmaxf(s[x][e], s[x][e + 2]);
+        top[x] = fmaxf(s[x][e], s[x][e + 2]);
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        m = fmaxf(m, top);
-        M = fmaxf(M, top + lv[x]);
+        for (int off = 4; off < 32; off <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], off));
+        m = fmaxf(m, top[x]);
       }
-      const float fl = ex2(a.m[0][e] - m), fo = ex2(a.M[0][e] - M);
+      const float by = a.m[0][e] - m;
+      float r = shifted(a.r[0][e], by);
+#pragma unroll
+      for (int x = 0; x < H; ++x) r = fmaxf(r, top[x] - m + lv[x]);
+      const float fl = ex2(by), fo = ex2(a.r[0][e] + by - r);
       a.m[0][e] = m;
-      a.M[0][e] = M;
+      a.r[0][e] = r;
       a.l[0][e] *= fl;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -425,14 +438,20 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
     }
   }
   uint32_t pb[H][2];
-  const float m0 = a.m[0][0], m1 = a.m[0][1], M0 = a.M[0][0], M1 = a.M[0][1];
 #pragma unroll
   for (int x = 0; x < H; ++x) {
-    a.l[0][0] += ex2(s[x][0] - m0) + ex2(s[x][2] - m0);
-    a.l[0][1] += ex2(s[x][1] - m1) + ex2(s[x][3] - m1);
-    const float f0 = lv[x] - M0, f1 = lv[x] - M1;
-    pb[x][0] = movmatrix_trans(pack_f16x2(ex2(s[x][0] + f0), ex2(s[x][1] + f1)));
-    pb[x][1] = movmatrix_trans(pack_f16x2(ex2(s[x][2] + f0), ex2(s[x][3] + f1)));
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[x][e] -= a.m[0][e & 1];
+      y[e] = s[x][e] + lv[x] - a.r[0][e & 1];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+    a.l[0][0] += ex2(s[x][0]) + ex2(s[x][2]);
+    a.l[0][1] += ex2(s[x][1]) + ex2(s[x][3]);
+    pb[x][0] = movmatrix_trans(pack_f16x2(y[0], y[1]));
+    pb[x][1] = movmatrix_trans(pack_f16x2(y[2], y[3]));
   }
   if (!tail) {
 #pragma unroll
@@ -474,8 +493,8 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
 // head_dim 64 half of the slices: warps w and w + 4 share dims).
 template <int D, int NG>
 __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, const Smem<D, NG>& sm,
-                                            const float* scales, uint32_t kt, uint32_t vt, int k, bool fresh, int first, int len,
-                                            int position, int chain, int chunk, int warp, int lane) {
+                                            const float* scales, uint32_t kt, uint32_t vt, int k, bool fresh, int first,
+                                            int len, int position, int chain, int chunk, int warp, int lane) {
   using S = Smem<D, NG>;
   const int g = lane >> 2, c = lane & 3;
   const int slice = first + warp * 16;
@@ -514,24 +533,26 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (!sees(slice + g + (e >> 1) * 8, len, position, token(n * 8 + 2 * c + (e & 1)), chain)) hidden |= 1u << (n * 4 + e);
+        if (!sees(slice + g + (e >> 1) * 8, len, position, token(n * 8 + 2 * c + (e & 1)), chain))
+          hidden |= 1u << (n * 4 + e);
   }
   // The slice's weights, into this warp's half of its pair's fragments
   uint2* weights =
       reinterpret_cast<uint2*>(sm.weights + k % 2 * (S::kWeights / 2)) + warp / 2 * NG * 64 + lane * 2 + warp % 2;
   float l[NG][2];
-  // Weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile.
+  // Weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile. They
+  // move once at most: they are worked out with the same roundings as x and y, which are monotone, so that no
+  // x or y is above 0 then (a product fused into x would break that where scores round by more than 8).
   for (;; fresh = false) {
     if (!fresh) {
       float top = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float x[4], y[4];  // s - m and s + log2 vs - M
+        float x[4], y[4];  // s - m and s - m + log2 vs - r
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float by = a.qs[n][e & 1] * ks;
-          x[e] = fmaf(s[n][e], by, -a.m[n][e & 1]);
-          y[e] = fmaf(s[n][e], by, lv - a.M[n][e & 1]);
+          x[e] = __fmul_rn(s[n][e], a.qs[n][e & 1] * ks) - a.m[n][e & 1];
+          y[e] = x[e] + lv - a.r[n][e & 1];
         }
         if (hidden != 0) {
 #pragma unroll
@@ -540,13 +561,16 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(x[e], y[e]));
-        weights[n * 64] = make_uint2(movmatrix_trans(pack_f16x2(ex2(y[0]), ex2(y[1]))),
-                                     movmatrix_trans(pack_f16x2(ex2(y[2]), ex2(y[3]))));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+        weights[n * 64] = make_uint2(movmatrix_trans(pack_f16x2(y[0], y[1])), movmatrix_trans(pack_f16x2(y[2], y[3])));
         l[n][0] = ex2(x[0]) + ex2(x[2]);
         l[n][1] = ex2(x[1]) + ex2(x[3]);
       }
-      if (!consumers_any<NG>(top > kSlack)) break;
+      if (!consumers_any<NG>(top > kSlack && sm.misc[4 + warp] != k + 1)) break;
     }
+    if (lane == 0) sm.misc[4 + warp] = k + 1;  // once a tile, whatever the scores
+    __syncwarp();
     // [warp][column], where the last tile's weights were: everyone has multiplied by them (a run's first
     // tile: start_unit)
     float2* tops = reinterpret_cast<float2*>(sm.weights + (k + 1) % 2 * (S::kWeights / 2));
@@ -555,30 +579,41 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float by = a.qs[n][e] * ks;
-        float top = fmaxf(hidden >> (n * 4 + e) & 1 ? -INFINITY : s[n][e] * by,
-                          hidden >> (n * 4 + e + 2) & 1 ? -INFINITY : s[n][e + 2] * by);
+        float top = fmaxf(hidden >> (n * 4 + e) & 1 ? -INFINITY : __fmul_rn(s[n][e], by),
+                          hidden >> (n * 4 + e + 2) & 1 ? -INFINITY : __fmul_rn(s[n][e + 2], by));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        if (g == 0) tops[warp * NG * 8 + n * 8 + 2 * c + e] = make_float2(top, top + lv);
+        if (g == 0) tops[warp * NG * 8 + n * 8 + 2 * c + e] = make_float2(top, lv);
       }
     consumers_sync<NG>();
-    float2 top = make_float2(-INFINITY, -INFINITY);  // of column `lane`
+    // of column `lane`: its m, which becomes the largest score if that is larger, and the largest score - m +
+    // log2 vs, with the roundings of the loop above
+    float m_lane = kNone, r_lane = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float m = __shfl_sync(0xffffffffu, a.m[n][e], (lane & 7) >> 1);
+        if (lane / 8 == n && lane % 2 == e) m_lane = m;
+      }
     if (lane < NG * 8) {
+#pragma unroll
+      for (int w = 0; w < kConsumers<NG>; ++w) m_lane = fmaxf(m_lane, tops[w * NG * 8 + lane].x);
 #pragma unroll
       for (int w = 0; w < kConsumers<NG>; ++w) {
         const float2 t = tops[w * NG * 8 + lane];
-        top = make_float2(fmaxf(top.x, t.x), fmaxf(top.y, t.y));
+        r_lane = fmaxf(r_lane, t.x - m_lane + t.y);
       }
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float m = fmaxf(a.m[n][e], __shfl_sync(0xffffffffu, top.x, n * 8 + 2 * c + e));
-        const float M = fmaxf(a.M[n][e], __shfl_sync(0xffffffffu, top.y, n * 8 + 2 * c + e));
-        const float fl = ex2(a.m[n][e] - m), fo = ex2(a.M[n][e] - M);
+        const float m = __shfl_sync(0xffffffffu, m_lane, n * 8 + 2 * c + e), by = a.m[n][e] - m;
+        const float r = fmaxf(shifted(a.r[n][e], by), __shfl_sync(0xffffffffu, r_lane, n * 8 + 2 * c + e));
+        const float fl = ex2(by), fo = ex2(a.r[n][e] + by - r);
         a.m[n][e] = m;
-        a.M[n][e] = M;
+        a.r[n][e] = r;
         a.l[n][e] *= fl;
         a.o[n][0][e] *= fo;
         a.o[n][0][e + 2] *= fo;
@@ -661,7 +696,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
   }
 }
 
-// Sums the consumer warps' states in warp order: sink(in_chunk, d, O, M, m, l) for every live column and
+// Sums the consumer warps' states in warp order: sink(in_chunk, d, O, r, m, l) for every live column and
 // dim.
 template <int D, typename Sink>
 __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& sm, int members, int warp, int lane,
@@ -678,7 +713,7 @@ __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& s
       for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
       if (g == 0) {
         float* st = red_stats + (warp * NG * 8 + n * 8 + 2 * c + e) * 3;
-        st[0] = a.M[n][e], st[1] = a.m[n][e], st[2] = l;
+        st[0] = a.r[n][e], st[1] = a.m[n][e], st[2] = l;
       }
     }
 #pragma unroll
@@ -697,20 +732,19 @@ __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& s
     for (int e0 = 0; e0 < 8 * (D / 2); e0 += kWarps * 32) {
       const int e = e0 + tid, col = e / (D / 2), d = e % (D / 2), in_chunk = n * 8 + col;
       if (in_chunk >= members) break;
-      float wM[kWarps], wm[kWarps], M = kNone, m = kNone;
+      const float* st = red_stats + in_chunk * 3;
+      float m = kNone, r = kNone, O = 0.f, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, st[w * NG * 24 + 1]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) r = fmaxf(r, st[w * NG * 24] + (st[w * NG * 24 + 1] - m));
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float* st = red_stats + (w * NG * 8 + in_chunk) * 3;
-        M = fmaxf(M, wM[w] = st[0]);
-        m = fmaxf(m, wm[w] = st[1]);
+        const float by = st[w * NG * 24 + 1] - m;
+        O += red_o[(w * (D / 2) + d) * 8 + col] * ex2(st[w * NG * 24] + by - r);
+        l += st[w * NG * 24 + 2] * ex2(by);
       }
-      float O = 0.f, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        O += red_o[(w * (D / 2) + d) * 8 + col] * ex2(wM[w] - M);
-        l += red_stats[(w * NG * 8 + in_chunk) * 3 + 2] * ex2(wm[w] - m);
-      }
-      sink(in_chunk, k0 * 16 + d, O, M, m, l);
+      sink(in_chunk, k0 * 16 + d, O, r, m, l);
     }
   }
 }
@@ -719,14 +753,14 @@ __device__ __forceinline__ void reduce_warps(State<D, 1>& a, const Smem<D, 1>& s
 template <int D, int NG>
 struct Totals {
   float* l;        // [warp][column]: denominators of the warp's slices
-  float2* pivots;  // [column]: M, m
-  float4* stats;   // [column]: M, m, l
+  float2* pivots;  // [column]: r, m
+  float4* stats;   // [column]: r, m, l
   __device__ Totals(const Smem<D, NG>& sm, int k) {
     l = reinterpret_cast<float*>(sm.weights + k % 2 * (Smem<D, NG>::kWeights / 2));
     pivots = reinterpret_cast<float2*>(l + kConsumers<NG> * NG * 8);
     stats = reinterpret_cast<float4*>(pivots + NG * 8);
   }
-  // A column's M, m and l, summed in warp order.
+  // A column's r, m and l, summed in warp order.
   __device__ float4 column(int col) const {
     float sum = 0.f;
 #pragma unroll
@@ -737,8 +771,8 @@ struct Totals {
 
 // Each warp ends with O of its dims; with head_dim 64 the first of the two that share dims.
 template <int D, int NG>
-__device__ __forceinline__ void join_warps(State<D, NG>& a, const Smem<D, NG>& sm, const Totals<D, NG>& totals, int warp,
-                                           int lane) {
+__device__ __forceinline__ void join_warps(State<D, NG>& a, const Smem<D, NG>& sm, const Totals<D, NG>& totals,
+                                           int warp, int lane) {
   constexpr int kChunks = D / 16;
   const int g = lane >> 2, c = lane & 3;
   float4* other = reinterpret_cast<float4*>(sm.red_o) + warp % kChunks * NG * 32 + lane;
@@ -751,7 +785,7 @@ __device__ __forceinline__ void join_warps(State<D, NG>& a, const Smem<D, NG>& s
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
       if (g == 0) totals.l[warp * NG * 8 + col] = l;
-      if (g == 0 && warp == 0) totals.pivots[col] = make_float2(a.M[n][e], a.m[n][e]);
+      if (g == 0 && warp == 0) totals.pivots[col] = make_float2(a.r[n][e], a.m[n][e]);
     }
     if (warp >= kChunks) other[n * 32] = make_float4(a.o[n][0][0], a.o[n][0][1], a.o[n][0][2], a.o[n][0][3]);
   }
@@ -784,9 +818,8 @@ __device__ __forceinline__ __nv_bfloat16* out_row(const Params& p, int b, int h,
   return p.out + ((static_cast<size_t>(b) * p.tokens + t) * p.q_heads + head) * D;
 }
 template <int D>
-__device__ __forceinline__ void write_out(const Params& p, int b, int h, int member, int d, float O, float M, float m,
-                                          float l) {
-  out_row<D>(p, b, h, member)[d] = __float2bfloat16_rn(finished(O, M, m, l));
+__device__ __forceinline__ void write_out(const Params& p, int b, int h, int member, int d, float O, float r, float l) {
+  out_row<D>(p, b, h, member)[d] = __float2bfloat16_rn(finished(O, r, l));
 }
 
 template <int D, int NG>
@@ -798,7 +831,7 @@ __device__ __forceinline__ void init_barriers(const Smem<D, NG>& sm, const CUten
   fence_barrier_init();
   prefetch_tensormap(kmap);
   prefetch_tensormap(vmap);
-  sm.misc[3] = 0;
+  for (int i = 3; i < 4 + kSlices; ++i) sm.misc[i] = 0;
 }
 
 // Producer warp: tile j of `pair` into stage k % stages. False after an abort.
@@ -842,8 +875,9 @@ __device__ __forceinline__ void drain(const Smem<D, NG>& sm, int issued) {
 // Consumer warp: tile j of a row with `len` slots from stage k % stages. After an abort the barriers
 // that follow are still taken, on whatever the stage holds.
 template <int D, int NG>
-__device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>& sm, const Params& p, int k, bool fresh, int j,
-                                             int len, int position, int chain, int chunk, int warp, int lane) {
+__device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>& sm, const Params& p, int k,
+                                             bool fresh, int j, int len, int position, int chain, int chunk, int warp,
+                                             int lane) {
   using S = Smem<D, NG>;
   const int s = k % S::kStages;
   if (sm.misc[3] == 0 && !mbar_wait_bounded(&sm.full[s], (k / S::kStages) & 1)) {
@@ -852,8 +886,8 @@ __device__ __forceinline__ void consume_tile(State<D, NG>& a, const Smem<D, NG>&
   }
   __syncwarp();
   const uint32_t kt = smem_u32(sm.ring + s * 2 * S::kTileBytes);
-  attend_tile(a, p, sm, sm.scales + s * kScales, kt, kt + S::kTileBytes, k, fresh, j * kTile, len, position, chain, chunk, warp,
-              lane);
+  attend_tile(a, p, sm, sm.scales + s * kScales, kt, kt + S::kTileBytes, k, fresh, j * kTile, len, position, chain,
+              chunk, warp, lane);
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.empty[s]);
 }
@@ -900,9 +934,9 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
   // values of an owner: an even number, so that pairs stay together; e / share for e < 2^16
   const int total = members * D, share = (total + 2 * C - 1) / (2 * C) * 2;
   const uint32_t magic = (0xffffffffu / share) + 1;
-  auto push_stats = [&](int col, int to, float M, float m, float l) {
+  auto push_stats = [&](int col, int to, float r, float m, float l) {
     const uint32_t at = map_shared(smem_u32(sm.recv_stats + (rank * NG * 8 + col) * 3), to);
-    st_cluster_f32(at, M);
+    st_cluster_f32(at, r);
     st_cluster_f32(at + 4, m);
     st_cluster_f32(at + 8, l);
   };
@@ -912,9 +946,9 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
   };
   if constexpr (NG == 1) {
     cluster_wait();  // every CTA of the cluster runs
-    reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float M, float m, float l) {
+    reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float r, float m, float l) {
       st_cluster_f32(push_to(col * D + d), O);
-      if (d < C) push_stats(col, d, M, m, l);  // one thread per rank passes this column's statistics on
+      if (d < C) push_stats(col, d, r, m, l);  // one thread per rank passes this column's statistics on
     });
   } else {
     const Totals<D, NG> totals(sm, count);
@@ -929,26 +963,27 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
     }
   }
   cluster_sync();  // every partial has landed; nobody touches another CTA's memory after this
-  // a rank's weight in a column's output, in place of its M; a column that sees nothing, or only zero
+  // a rank's weight in a column's output, in place of its r; a column that sees nothing, or only zero
   // values, is marked by l = 0
   for (int c0 = 0; c0 < NG * 8; c0 += kWarps * 2) {
     const int col = c0 + static_cast<int>(threadIdx.x) / 16, q = threadIdx.x & 15;
     static_assert(kMaxCluster == 16, "a rank per lane of half a warp");
     const bool on = col < members && q < C;
     float* st = sm.recv_stats + (q * NG * 8 + col) * 3;
-    const float M_q = on ? st[0] : kNone, m_q = on ? st[1] : kNone;
-    float M = M_q, m = m_q;
+    const float r_q = on ? st[0] : kNone, m_q = on ? st[1] : kNone;
+    float m = m_q;
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) {
-      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    }
-    float l = on ? st[2] * ex2(m_q - m) : 0.f;
+    for (int off = 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float by = m_q - m;
+    float r = shifted(r_q, by);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, off));
+    float l = on ? st[2] * ex2(by) : 0.f;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     if (on) {
-      st[0] = ex2(M_q - M) * finished(1.f, M, m, l);
-      st[2] = M == kNone && l > 0.f ? 0.f : l;
+      st[0] = ex2(r_q + by - r) * finished(1.f, r, l);
+      st[2] = r == kNone && l > 0.f ? 0.f : l;
     }
   }
   consumers_sync<NG>();
@@ -1073,12 +1108,12 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
     const int members = min(p.width, p.members - chunk * p.width);
     if constexpr (NG == 1) {
       consumers_sync<NG>();  // the last run's reductions are read
-      reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float M, float m, float l) {
+      reduce_warps(a, sm, members, warp, lane, [&](int col, int d, float O, float r, float m, float l) {
         if (whole) {
-          write_out<D>(p, run_b, h, chunk * p.width + col, d, O, M, m, l);
+          write_out<D>(p, run_b, h, chunk * p.width + col, d, O, r, l);
         } else {
           p.acc[(slot * p.width + col) * D + d] = O;
-          if (d == 0) p.stats[slot * p.width + col] = make_float4(M, m, l, 0.f);
+          if (d == 0) p.stats[slot * p.width + col] = make_float4(r, m, l, 0.f);
         }
       });
     } else {
@@ -1095,8 +1130,9 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
       each_pair(a, members, warp, lane, [&](int col, int d, float O0, float O1) {
         if (whole) {
           const float4 st = totals.stats[col];
-          *reinterpret_cast<__nv_bfloat162*>(out_row<D>(p, run_b, h, chunk * p.width + col) + d) = __floats2bfloat162_rn(
-              finished(O0, st.x, st.y, st.z), finished(O1, st.x, st.y, st.z));
+          __nv_bfloat16* out = out_row<D>(p, run_b, h, chunk * p.width + col) + d;
+          *reinterpret_cast<__nv_bfloat162*>(out) =
+              __floats2bfloat162_rn(finished(O0, st.x, st.z), finished(O1, st.x, st.z));
         } else {
           *reinterpret_cast<float2*>(p.acc + (slot * p.width + col) * D + d) = make_float2(O0, O1);
         }
@@ -1140,14 +1176,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   if (n > 0 && lo == hi) return;  // one run covered the unit and wrote its output
   for (int e = threadIdx.x; e < members * D; e += kMergeThreads) {
     const int col = col0 + e / D, d = e % D;
-    float M = kNone, m = kNone, O = 0.f, l = 0.f;
+    float r = kNone, m = kNone, O = 0.f, l = 0.f;
     if (n > 0) {
       const float4* st = p.stats + (static_cast<size_t>(lo) + blockIdx.x) * p.width + col;
       const float* acc = p.acc + ((static_cast<size_t>(lo) + blockIdx.x) * p.width + col) * D + d;
       for (int i0 = 0; i0 <= hi - lo; i0 += kMergeRuns) {
         float4 s[kMergeRuns];
         float v[kMergeRuns];
-        float tM = M, tm = m;
+        float to_m = m;
 #pragma unroll
         for (int i = 0; i < kMergeRuns; ++i) {
           const int run = i0 + i;
@@ -1157,22 +1193,22 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
           v[i] = on ? __ldcg(acc + static_cast<size_t>(run) * p.width * D) : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < kMergeRuns; ++i) {
-          tM = fmaxf(tM, s[i].x);
-          tm = fmaxf(tm, s[i].y);
-        }
-        O *= ex2(M - tM);
-        l *= ex2(m - tm);
-        M = tM;
-        m = tm;
+        for (int i = 0; i < kMergeRuns; ++i) to_m = fmaxf(to_m, s[i].y);
+        float to_r = shifted(r, m - to_m);
+#pragma unroll
+        for (int i = 0; i < kMergeRuns; ++i) to_r = fmaxf(to_r, s[i].x + (s[i].y - to_m));
+        O *= ex2(r + (m - to_m) - to_r);
+        l *= ex2(m - to_m);
+        r = to_r;
+        m = to_m;
 #pragma unroll
         for (int i = 0; i < kMergeRuns; ++i) {
-          O += v[i] * ex2(s[i].x - M);
+          O += v[i] * ex2(s[i].x + (s[i].y - m) - r);
           l += s[i].z * ex2(s[i].y - m);
         }
       }
     }
-    write_out<D>(p, b, h, chunk * p.width + col, d, O, M, m, l);
+    write_out<D>(p, b, h, chunk * p.width + col, d, O, r, l);
   }
 }
 
@@ -1285,7 +1321,8 @@ int launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int cl
   const int units = p.batch * p.kv_heads * p.chunks;
   constexpr int bytes = Smem<D, NG>::kTotal;
   if (cluster > 0)
-    return launch_ex(cluster_kernel<D, NG>, dim3(cluster, units), dim3(kThreads<NG>), bytes, stream, cluster, km, vm, p);
+    return launch_ex(cluster_kernel<D, NG>, dim3(cluster, units), dim3(kThreads<NG>), bytes, stream, cluster, km, vm,
+                     p);
   const int st = launch_ex(persistent_kernel<D, NG>, dim3(p.ctas), dim3(kThreads<NG>), bytes, stream, 1, km, vm, p);
   if (st != FB_OK) return st;
   return launch_ex(merge_kernel<D>, dim3(units, (p.width + 7) / 8), dim3(kMergeThreads), 0, stream, 1, p);

@@ -126,23 +126,6 @@ __device__ __forceinline__ void load_packed8(const AppendParams& p, size_t off, 
   for (int e = 0; e < kE; ++e) x[e] = bf16_round(x[e]);
 }
 
-// Two fp32 operations in one instruction (sm_100): a prompt is bound by issue.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; "
-      "fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z; }"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-
 // gain * cos and the partner's -+ gain * sin of a lane's dims, in pairs: RoPE of x * inv * gain is then
 // inv * (x c + partner s).
 struct Rotation {
@@ -538,7 +521,8 @@ extern "C" int fb_qk_norm_rope_append_q8(const void* packed, int packed_splits, 
   p.query_ctas = static_cast<int>(query_ctas);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    return packed_splits ? q8::launch_append<128, true>(p, rows, ctas, s) : q8::launch_append<128, false>(p, rows, ctas, s);
+    return packed_splits ? q8::launch_append<128, true>(p, rows, ctas, s)
+                         : q8::launch_append<128, false>(p, rows, ctas, s);
   return packed_splits ? q8::launch_append<64, true>(p, rows, ctas, s) : q8::launch_append<64, false>(p, rows, ctas, s);
 }
 

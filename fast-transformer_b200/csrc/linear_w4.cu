@@ -1,25 +1,29 @@
 // Projections with 4-bit weights and group scales, y[M, N] = x[M, K] @ W[N, K]^T for M <= 64 rows,
 // W[n, k] = code[n, k] * scale[n, k / group], codes -8..7 (sm_100a, tcgen05).
 //
-// Bound by the packed codes (N K / 2 bytes), and close behind by their unpacking, which is why the
+// Bound by the packed codes (N K / 2 bytes) and, as built, by their unpacking (0.13 us of the ALU pipe for a
+// block of 128 x 128 codes, which arrives in 0.19 us of an SM's share of the bandwidth), which is why the
 // products leave the warps altogether: a thread owns one of a tile's 128 weight rows, unpacks its
 // codes to bf16 and stores them to tensor memory, where they are the A operand of
 // tcgen05.mma (D[128 x M'] += A[128 x 16] B[16 x M'], B = x in shared memory, M' = M padded to 16,
 // 32 or 64). Each scale group accumulates in its own D columns; the thread that owns the row reads
 // them back, multiplies by its scale in fp32 and adds them to its row's totals in registers. (A
-// first form with mma.sync spent twice the instructions on fragments, addends and scaling: 20.4 us
-// for 24576 x 4096 at M = 16 whatever its warps, tiles and stages.)
+// first form with mma.sync spent twice the instructions on fragments, addends and scaling.)
+//
+// Measured (us, GB/s of codes and scales): 24576 x 4096, group 128, M = 16 20.7, 2.5 TB/s (without the
+// conversion it would take 15.7, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
+// merge); 4096 x 12288, group 32, M = 5 12.0, 2.4 TB/s; 6144 x 4096, M = 64 11.9; 4096 x 1024, group 64, M = 1 4.7.
 //
 // Unpacking is exact: a nibble q = code + 8 in the low mantissa bits of 128.0 is the bf16 number
 // 128 + q; subtracting 136 leaves the code. W itself is never rounded, x stays bf16.
 //
 // Work: a cluster of `splits` CTAs owns a 128-row tile and cuts its 128-column blocks into equal
 // contiguous ranges, one per CTA. (Clusters of several tiles, for evener waves, gained 9% at 24576 x 4096
-// and lost 15% at small sizes.) The
-// packed layout keeps a block's codes and scales together, so a block is one bulk copy (8 KB and
-// 256 bytes a group) and two boxes of x. Warp roles: four unpacking warps, a producer lane, an MMA
-// lane; A is double-buffered and block b is unpacked while block b - 1 multiplies. The CTAs' totals
-// are pushed to the owner of each output through distributed shared memory and added in rank order:
+// and lost 15% at small sizes.) The packed layout keeps a block's codes and scales together, so a block is
+// one bulk copy (8 KB and 256 bytes a group) and two boxes of x. Warp roles: two sets of four unpacking warps
+// that take parts in turn, each with its A and D, a producer and an MMA warp, whose issue sits behind
+// elect.sync (behind `lane == 0` it took four times as long). Up to 32 rows two CTAs share an SM. The CTAs'
+// totals are pushed to the owner of each output through distributed shared memory and added in rank order:
 // one launch, no workspace, the same bits every time, and the result leaves finished (bf16, fp32
 // or SwiGLU).
 #include <cuda_bf16.h>
@@ -450,10 +454,12 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* packed, 
     const Word w(i, l);
     if (w.row >= n) continue;
     const uint32_t word = *reinterpret_cast<const uint32_t*>(packed + w.at);
-    const float f = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(packed + scale_at(l, w.row, w.col >> l.group_shift)));
+    const float f = __bfloat162float(
+        *reinterpret_cast<const __nv_bfloat16*>(packed + scale_at(l, w.row, w.col >> l.group_shift)));
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>((word >> (4 * (e / 2) + 16 * (e & 1))) & 15u) - 8) * f;
+    for (int e = 0; e < 8; ++e)
+      v[e] = static_cast<float>(static_cast<int>((word >> (4 * (e / 2) + 16 * (e & 1))) & 15u) - 8) * f;
     *reinterpret_cast<uint4*>(out + static_cast<size_t>(w.row) * l.k + w.col) =
         make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
   }
@@ -551,7 +557,8 @@ extern "C" size_t fb_w4_packed_bytes(int n, int k, int group) {
   return l.tiles * l.tile_bytes;
 }
 
-extern "C" int fb_w4_pack(const int8_t* codes, const void* scales, void* packed, int n, int k, int group, void* stream) {
+extern "C" int fb_w4_pack(const int8_t* codes, const void* scales, void* packed, int n, int k, int group,
+                          void* stream) {
   if (!codes || !scales || !packed) return FB_ERR_ARG;
   if (!w4::valid(n, k, group)) return FB_ERR_SHAPE;
   return launch_ex(w4::pack_kernel, dim3(sm_count() * 8), dim3(256), 0, static_cast<cudaStream_t>(stream), 1, codes,

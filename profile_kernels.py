@@ -192,7 +192,8 @@ def step(args):
         end.synchronize()
         ms = start.elapsed_time(end) / 20
         print(f"step {args.preset} {args.kv_cache} cache, {'4-bit' if args.weight_group else 'bf16'} weights, "
-              f"TP-shard 1/{args.tp_size} B={args.batch} L={args.length}: {ms * 1e3:.1f} us per captured step ({args.batch / ms * 1e3:.0f} tok/s for this shard alone)")
+              f"TP-shard 1/{args.tp_size} B={args.batch} L={args.length}: {ms * 1e3:.1f} us per captured step "
+              f"({args.batch / ms * 1e3:.0f} tok/s for this shard alone)")
         state.release()
         return
     torch.cuda.nvtx.range_push("profiled")

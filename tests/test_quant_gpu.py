@@ -156,6 +156,42 @@ def test_decode_attention_query_range(factor):
     check_attention(decode_attention_q8(query.to(DEV), handle(cache), position.to(DEV), scale), expect, bound)
 
 
+@pytest.mark.parametrize("tokens,dim,batch", [(1, 128, 2), (1, 64, 40), (3, 128, 2), (5, 64, 40), (8, 128, 40)])
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 60])
+def test_scores_whose_rounding_passes_one(tokens, dim, batch, factor):
+    """Scores of 2^24 and more: the softmax is one slot, whose value comes back (each bf16 once rounded). Value
+    scales far from 1 and in every block another must not turn the scores' rounding into a factor."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(tokens + batch)
+    capacity, kv_heads, groups = 300, 4, 4
+    cache = oq.random_cache(batch, kv_heads, capacity, dim, 16, g)
+    blocks = cache["value_scales"].shape[2]
+    cache["value_scales"] *= torch.exp2(torch.randint(-40, 40, (batch, kv_heads, blocks), generator=g).float())
+    position = torch.randint(130, capacity - tokens, (batch,), generator=g)
+    chain = torch.full((batch,), tokens)
+    query = (torch.randn(batch, tokens, kv_heads * groups, dim, generator=g) * factor).bfloat16()
+    out = block_attention_q8(query.to(DEV), handle(cache), position.to(DEV), 1.0, chain.to(DEV)).cpu().double()
+    keys, values = (cache[name + "s"].double() * cache[name + "_scales"].double().repeat_interleave(
+        16, 2)[:, :, :capacity, None] for name in ("key", "value"))
+    checked = 0
+    for b in range(batch):
+        for t in range(tokens):
+            n = int(position[b]) + t + 1
+            q = query[b, t].double().view(kv_heads, groups, dim)
+            scores = torch.einsum("hgd,hnd->hgn", q, keys[b, :, :n])
+            best = scores.topk(2, -1)
+            # fp32 sums of at most 128 exact products, then two roundings: 2^-15 of the two scores' sizes
+            size = torch.einsum("hgd,hnd->hgn", q.abs(), keys[b, :, :n].abs()).amax(-1)
+            clear = best.values[..., 0] - best.values[..., 1] > 2.0 ** -15 * size + 200
+            expect = torch.gather(values[b, :, :n], 1, best.indices[..., :1].expand(-1, -1, dim))
+            got = out[b, t].view(kv_heads, groups, dim)
+            # P and the output round once each
+            assert ((got - expect).abs() <= (2.0 ** -8 + 2.0 ** -10) * expect.abs())[clear].all(), (b, t)
+            checked += int(clear.sum())
+    assert checked > batch * tokens * kv_heads * groups // 2
+    assert torch.isfinite(out).all()
+
+
 def test_decode_attention_passes_nan_on():
     """A NaN in a slot that a row sees reaches that row's outputs, and no other row's."""
     from kernels.decode_attention import decode_attention_q8
