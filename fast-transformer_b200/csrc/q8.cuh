@@ -54,7 +54,7 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// Two fp32 operations in one instruction (sm_100), each rounded by itself.
+// Two fp32 operations in one instruction (sm_100).
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"

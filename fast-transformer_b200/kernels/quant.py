@@ -131,8 +131,8 @@ def pack_weight4(codes, scales):
     group = k // scales.shape[1]
     _check_shape(n, k, group)
     _native.require_device(codes.device, codes, scales)
-    low, high = torch.aminmax(codes)
-    if int(low) < -8 or int(high) > 7:
+    low, high = torch.stack(torch.aminmax(codes)).tolist()
+    if low < -8 or high > 7:
         raise ValueError("4-bit codes lie in -8..7")
     codes, scales = codes.contiguous(), scales.contiguous()
     packed = torch.empty(int(lib.fb_w4_packed_bytes(n, k, group)), dtype=torch.uint8, device=codes.device)
@@ -152,6 +152,8 @@ def quantize_weight4(weight, group=128):
     _native.require_device(weight.device, weight)
     parts = weight.float().reshape(n, k // group, group)
     scales = (parts.abs().amax(-1) / 7.0).to(torch.bfloat16)
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError("quantize_weight4 takes finite weights")
     divisor = torch.where(scales == 0, torch.ones_like(scales), scales).float()
     codes = (parts / divisor[..., None]).round().clamp_(-8, 7).to(torch.int8).reshape(n, k)
     return pack_weight4(codes, scales)

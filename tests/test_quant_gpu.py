@@ -640,6 +640,24 @@ def test_quantize_weight4_is_nearest():
     assert (w.view(48, 4, 64)[3, 1] == 0).all()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_quantize_weight4_refuses_what_is_not_finite(bad):
+    from kernels.quant import quantize_weight4
+    weight = torch.ones(16, 128, dtype=torch.bfloat16, device=DEV)
+    weight[9, 70] = bad
+    with pytest.raises(ValueError):
+        quantize_weight4(weight, 64)
+
+
+@pytest.mark.parametrize("code", [-9, 8])
+def test_pack_weight4_refuses_codes_out_of_range(code):
+    from kernels.quant import pack_weight4
+    codes = torch.zeros(8, 64, dtype=torch.int8, device=DEV)
+    codes[7, 63] = code
+    with pytest.raises(ValueError):
+        pack_weight4(codes, torch.ones(8, 1, dtype=torch.bfloat16, device=DEV))
+
+
 @pytest.mark.parametrize("rows", [65, 100, 128, 129, 300])
 def test_linear_more_rows_than_a_launch_takes(rows):
     """Two launches up to 128 rows, expanded weights above (rounded once to bf16: 2^-8 of each product)."""
@@ -695,3 +713,37 @@ def test_calls_on_two_streams_at_once():
         for run in runs:
             for a, b in zip(want, run):
                 assert torch.equal(a, b)
+
+
+def test_first_calls_of_a_shape_inside_a_capture():
+    """Shapes that no eager call has met: captured, replayed on new inputs, equal to eager calls after it."""
+    from kernels.decode_attention import block_attention_q8, decode_attention_q8
+    from kernels.linear import linear
+    from kernels.quant import quantize_weight4
+    g = torch.Generator().manual_seed(41)
+    cache = handle(oq.random_cache(37, 8, 5200, 64, 32, g))  # the persistent form: a workspace of the graph's pool
+    w = quantize_weight4(torch.randn(264, 416, generator=g).bfloat16().to(DEV), 32)
+    x = torch.randn(3, 416, generator=g).bfloat16().to(DEV)
+    q = torch.randn(37, 2, 24, 64, generator=g).bfloat16().to(DEV)
+    position = torch.randint(-1, 5198, (37,), generator=g).to(DEV)
+    chain = torch.full((37,), 2).to(DEV)
+    one = q[:, :1].transpose(1, 2).contiguous()
+
+    def calls():
+        return (linear(x, w), decode_attention_q8(one, cache, position, 0.125),
+                block_attention_q8(q, cache, position, 0.125, chain))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = calls()
+    for seed in range(2):
+        x.copy_(torch.randn(3, 416, generator=g).bfloat16())
+        one.copy_(torch.randn(37, 24, 1, 64, generator=g).bfloat16())
+        q.copy_(torch.randn(37, 2, 24, 64, generator=g).bfloat16())
+        position.copy_(torch.randint(-1, 5198, (37,), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, calls()):
+            assert torch.equal(a, b)
