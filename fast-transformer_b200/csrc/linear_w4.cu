@@ -10,8 +10,8 @@
 // them back, multiplies by its scale in fp32 and adds them to its row's totals in registers. (A
 // first form with mma.sync spent twice the instructions on fragments, addends and scaling.)
 //
-// Measured (us, GB/s of codes and scales): 24576 x 4096, group 128, M = 16 20.7, 2.5 TB/s (without the
-// conversion it would take 15.7, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
+// Measured (us, GB/s of codes and scales): 24576 x 4096, group 128, M = 16 19.9, 2.7 TB/s (without the
+// conversion about 15, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
 // merge); 4096 x 12288, group 32, M = 5 12.0, 2.4 TB/s; 6144 x 4096, M = 64 11.9; 4096 x 1024, group 64, M = 1 4.7.
 //
 // Unpacking is exact: a nibble q = code + 8 in the low mantissa bits of 128.0 is the bf16 number
@@ -176,10 +176,10 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
   const int splits = gridDim.x, rank = blockIdx.x;
   const int tile = blockIdx.y, blocks = p.layout.blocks();  // of a tile; this CTA: [b0, b0 + count)
   const int b0 = blocks * rank / splits, count = blocks * (rank + 1) / splits - b0;
-  const int parts = count * PARTS;  // part i: stage i / PARTS, columns_of(i) columns (none at a short block's end)
-  auto columns_of = [&](int i) {
-    return max(0, min(C::kPart, p.layout.columns(b0 + i / PARTS) - i % PARTS * C::kPart));
-  };
+  const int parts = count * PARTS;  // part i: stage i / PARTS % NS
+  // the row's last block may be short: its parts have tail_columns(which) columns, others kPart
+  const int short_block = p.layout.k % kBlock != 0 && b0 + count == blocks ? count - 1 : -1;
+  auto tail_columns = [&](int which) { return max(0, min(C::kPart, p.layout.k % kBlock - which * C::kPart)); };
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 
   if (warp == kProducerWarp) {
     const uint64_t policy = l2_evict_first_policy();
-    auto weights = [&](int i) {
-      const int s = i % NS, bytes = p.layout.bytes(b0 + i);
+    auto weights = [&](int i, int s) {
+      const int bytes = p.layout.bytes(b0 + i);
       const uint8_t* src = p.packed + p.layout.at(tile, b0 + i);
       if (elect_one()) {
         mbar_arrive_expect_tx(&full[s], bytes + C::kX);
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
       }
       __syncwarp();
     };
-    auto inputs = [&](int i) {
-      const int s = i % NS, column = (b0 + i) * kBlock;
+    auto inputs = [&](int i, int s) {
+      const int column = (b0 + i) * kBlock;
       uint8_t* at = ring + s * C::kStage;
       if (elect_one()) {
         tma_load_2d(at, &xmap, &full[s], column, 0);
@@ -236,14 +236,15 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     };
     // weights are static: the ring fills before the wait on the previous kernel
     const int pre = count < NS ? count : NS;
-    for (int i = 0; i < pre; ++i) weights(i);
+    for (int i = 0; i < pre; ++i) weights(i, i);
     pdl_wait();
-    for (int i = 0; i < pre; ++i) inputs(i);
+    for (int i = 0; i < pre; ++i) inputs(i, i);
     int i = pre;
-    for (; i < count; ++i) {
-      if (!__all_sync(0xffffffffu, wait(&empty[i % NS], ((i / NS) - 1) & 1, kErrTimeoutEmpty))) break;
-      weights(i);
-      inputs(i);
+    for (int s = 0, phase = 0; i < count; ++i) {  // stage i % NS, i / NS - 1 uses of it done
+      if (!__all_sync(0xffffffffu, wait(&empty[s], phase, kErrTimeoutEmpty))) break;
+      weights(i, s);
+      inputs(i, s);
+      if (++s == NS) s = 0, phase ^= 1;
     }
     if (*abort_flag != 0)  // copies in flight land before the CTA's shared memory is released
       for (int k = i > NS ? i - NS : 0; k < i; ++k) mbar_wait_bounded(&full[k % NS], (k / NS) & 1);
@@ -253,13 +254,14 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     constexpr uint32_t kIdesc = tc::idesc_bf16(kRows, M, false, false);
     constexpr int kPer = C::kPart / 16 / GROUPS;  // products of a group
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-    for (int i = 0; i < parts; ++i) {
-      const int j = i / PARTS, s = j % NS, set = i % kSets, turn = i / kSets, steps = columns_of(i) / 16;
+    const uint64_t ring_desc = tc::desc_sw128(smem_u32(ring), 16, 1024);
+    for (int i = 0, s = 0, turn = 0; i < parts; ++i) {
+      const int set = i % kSets;
+      const int steps = (i / PARTS == short_block ? tail_columns(i % PARTS) : C::kPart) / 16;
       // the set has seen this stage land, and read D of its last part, before it wrote A
-      if (!__all_sync(0xffffffffu, wait(&a_full[set], turn & 1, kErrTimeoutMma))) break;
+      if (!__all_sync(0xffffffffu, wait(&a_full[set], turn, kErrTimeoutMma))) break;
       tc::fence_after();
-      const uint32_t x = smem_u32(ring + s * C::kStage) + i % PARTS * C::kBoxBytes;
-      const uint64_t xdesc = tc::desc_sw128(x, 16, 1024);
+      const uint64_t xdesc = ring_desc + (s * C::kStage + i % PARTS * C::kBoxBytes) / 16;
       const uint32_t d = tmem_u + C::kD + set * GROUPS * M, a = tmem_u + set * C::kA;
       if (elect_one()) {
         if (steps == C::kPart / 16) {
@@ -276,6 +278,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         tc::commit(&d_full[set]);
       }
       __syncwarp();
+      if (set == kSets - 1) turn ^= 1;
+      if (i % PARTS == PARTS - 1 && ++s == NS) s = 0;
     }
     if (splits > 1) cluster_wait();
   } else {
@@ -287,20 +291,29 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     constexpr int kRuns = C::kPart / kRun;
     uint4 codes[kRuns];
     float scale[GROUPS];
+    // The set's parts set, set + kSets, ... lie kSets / PARTS stages apart; with two parts a block a set takes
+    // the same one of every block.
+    constexpr int kStageStep = kSets / PARTS;
+    const int which = PARTS == 1 ? 0 : set;
+    const int tail_groups = tail_columns(which) >> p.layout.group_shift;
+    const int tail_scales = p.layout.k % kBlock / kRun * kRunBytes;
+    int s = set / PARTS, phase = 0;  // of the next fetch
     // Part i's codes and scales to registers; this warp is then done with the stage.
     auto fetch = [&](int i) {
-      const int j = i / PARTS, s = j % NS, part = i % PARTS;
-      if (!__all_sync(0xffffffffu, wait(&full[s], (j / NS) & 1, kErrTimeoutFull))) return false;
+      if (!__all_sync(0xffffffffu, wait(&full[s], phase, kErrTimeoutFull))) return false;
       const uint8_t* at = ring + s * C::kStage + C::kX;
 #pragma unroll
       for (int r = 0; r < kRuns; ++r)  // runs and groups past the last block's columns read what is not used
-        codes[r] = *reinterpret_cast<const uint4*>(at + (part * kRuns + r) * kRunBytes + row * 16);
-      const uint8_t* scales = at + p.layout.columns(b0 + j) / kRun * kRunBytes + row * 2;
+        codes[r] = *reinterpret_cast<const uint4*>(at + (which * kRuns + r) * kRunBytes + row * 16);
+      const uint8_t* scales =
+          at + (i / PARTS == short_block ? tail_scales : kBlock / kRun * kRunBytes) + row * 2;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
-        scale[g] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(scales + (part * GROUPS + g) * kRows * 2));
+        scale[g] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(scales + (which * GROUPS + g) * kRows * 2));
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+      s += kStageStep;
+      if (s >= NS) s -= NS, phase ^= 1;
       return true;
     };
     const int share = (64 + splits - 1) / splits;  // features (rows f and f + 64) of an owner
@@ -310,8 +323,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     for (int m = 0; m < M; ++m) total[m] = 0.f;
     bool ok = set >= parts || fetch(set);
     if (splits > 1) cluster_wait();  // every CTA of the cluster runs
+    int turn = 0;
     for (int i = set; ok && i < parts; i += kSets) {  // this set's parts
-      const int turn = i / kSets, groups = columns_of(i) >> p.layout.group_shift;
+      const int groups = i / PARTS == short_block ? tail_groups : GROUPS;
       // A is free: the products of this set's last block were waited for below
 #pragma unroll
       for (int r = 0; r < kRuns; ++r) {
@@ -334,8 +348,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) f[g] = scale[g];
       ok = i + kSets >= parts || fetch(i + kSets);  // while the part multiplies
-      ok = ok && __all_sync(0xffffffffu, wait(&d_full[set], turn & 1, kErrTimeoutMma));
+      ok = ok && __all_sync(0xffffffffu, wait(&d_full[set], turn, kErrTimeoutMma));
       if (!ok) break;
+      turn ^= 1;
       tc::fence_after();
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
