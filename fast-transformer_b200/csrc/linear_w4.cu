@@ -12,7 +12,7 @@
 //
 // Measured (us, GB/s of codes and scales): 24576 x 4096, group 128, M = 16 19.9, 2.7 TB/s (without the
 // conversion about 15, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
-// merge); 4096 x 12288, group 32, M = 5 12.0, 2.4 TB/s; 6144 x 4096, M = 64 11.9; 4096 x 1024, group 64, M = 1 4.7.
+// merge); 4096 x 12288, group 32, M = 5 11.8, 2.4 TB/s; 6144 x 4096, M = 64 12.4; 4096 x 1024, group 64, M = 1 4.7.
 //
 // Unpacking is exact: a nibble q = code + 8 in the low mantissa bits of 128.0 is the bf16 number
 // 128 + q; subtracting 136 leaves the code. W itself is never rounded, x stays bf16.
