@@ -12,7 +12,10 @@
 // p'[c] = 2^(s[c] - m + log2 vs - r) with a pivot r of its own over s - m + log2 vs, so a block's scale
 // can neither overflow nor wash out P's f16 range, while the denominator sums 2^(s - m) in
 // fp32. r is kept relative to m: where scores are so large that their own rounding passes 1, the result is
-// still a mean of values. Q is scaled by a power of two to f16's range (exact for any bf16 row).
+// still a mean of values. r is set 7 below the largest exponent, so that P fills f16's range from the top and
+// weights down to 2^-32 of the largest count. (With r at the largest, those below 2^-25 of it became zero in
+// the numerator alone: all that stood behind one leading slot, however many, could be lost.) Q is scaled by a
+// power of two to f16's range (exact for any bf16 row).
 //
 // Bound by the bytes of codes. Members = the T * G query heads that share a KV head, in groups of
 // 8 NG columns; a unit = (row, KV head, member group); its tiles are 128 slots of K and V. A CTA is
@@ -53,7 +56,8 @@ constexpr int kThreads = (kConsumers<NG> + 1) * 32;
 constexpr int kMaxBatch = 1024;
 constexpr int kScales = 2 * kSlices;  // per stage: K and V scale of each 16-slot slice
 constexpr int kMaxCluster = 16;      // above 8: the non-portable cluster size attribute
-constexpr float kSlack = 8.f;        // log2 a score may pass the pivot by: p <= 2^8, exact enough in f16
+constexpr float kSlack = 8.f;        // log2 a score may pass the pivot by before it moves
+constexpr float kLift = 7.f;         // log2 of the largest p' when its pivot moves: p' <= 2^(kLift + kSlack), f16 ends at 65504
 
 struct Params {
   const __nv_bfloat16* q;  // [B, T, Hq, D]
@@ -409,7 +413,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
 #pragma unroll
     for (int x = 0; x < H; ++x) {
       const float over = fmaxf(s[x][e], s[x][e + 2]) - a.m[0][e];
-      moves = moves || fmaxf(over, over + lv[x] - a.r[0][e]) > kSlack;
+      moves = moves || over > kSlack || over + lv[x] - a.r[0][e] > kLift + kSlack;
     }
   if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
@@ -425,7 +429,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
       const float by = a.m[0][e] - m;
       float r = shifted(a.r[0][e], by);
 #pragma unroll
-      for (int x = 0; x < H; ++x) r = fmaxf(r, top[x] - m + lv[x]);
+      for (int x = 0; x < H; ++x) r = fmaxf(r, top[x] - m + lv[x] - kLift);
       const float fl = ex2(by), fo = ex2(a.r[0][e] + by - r);
       a.m[0][e] = m;
       a.r[0][e] = r;
@@ -541,11 +545,12 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
       reinterpret_cast<uint2*>(sm.weights + k % 2 * (S::kWeights / 2)) + warp / 2 * NG * 64 + lane * 2 + warp % 2;
   float l[NG][2];
   // Weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile. They
-  // move once at most: they are worked out with the same roundings as x and y, which are monotone, so that no
-  // x or y is above 0 then (a product fused into x would break that where scores round by more than 8).
+  // move once at most: they are worked out with the same roundings as x and y, which are monotone, so that no x is
+  // above 0 then and no y above 8, kLift rounded to a step of at most 8 (where steps are 16 and more it rounds to
+  // 0). A product fused into x would break that where scores round by more than 8.
   for (;; fresh = false) {
     if (!fresh) {
-      float top = 0.f;
+      float top = 0.f, top_y = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float x[4], y[4];  // s - m and s - m + log2 vs - r
@@ -560,14 +565,17 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
             if (hidden >> (n * 4 + e) & 1) x[e] = y[e] = -INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(x[e], y[e]));
+        for (int e = 0; e < 4; ++e) {
+          top = fmaxf(top, x[e]);
+          top_y = fmaxf(top_y, y[e]);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
         weights[n * 64] = make_uint2(movmatrix_trans(pack_f16x2(y[0], y[1])), movmatrix_trans(pack_f16x2(y[2], y[3])));
         l[n][0] = ex2(x[0]) + ex2(x[2]);
         l[n][1] = ex2(x[1]) + ex2(x[3]);
       }
-      if (!consumers_any<NG>(top > kSlack && sm.misc[4 + warp] != k + 1)) break;
+      if (!consumers_any<NG>((top > kSlack || top_y > kLift + kSlack) && sm.misc[4 + warp] != k + 1)) break;
     }
     if (lane == 0) sm.misc[4 + warp] = k + 1;  // once a tile, whatever the scores
     __syncwarp();
@@ -587,7 +595,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
       }
     consumers_sync<NG>();
     // of column `lane`: its m, which becomes the largest score if that is larger, and the largest score - m +
-    // log2 vs, with the roundings of the loop above
+    // log2 vs, with the roundings of the loop above, less kLift
     float m_lane = kNone, r_lane = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NG; ++n)
@@ -604,6 +612,7 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
         const float2 t = tops[w * NG * 8 + lane];
         r_lane = fmaxf(r_lane, t.x - m_lane + t.y);
       }
+      r_lane -= kLift;
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n)

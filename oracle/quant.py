@@ -53,7 +53,8 @@ def visible(position, tokens, chain, t, capacity):
 def attention(query, cache, position, scale, chain=None):
     """query [B, T, Hq, D] -> (out, bound) in 64 bits. ``bound``: how far a bf16 result may be off that
     sums in fp32 and rounds P (scaled by V's block scale against its largest) to f16:
-      2^-8 |out|  (the output) + sum_c max(2^-11 p'_c, 2^-25) |vcode_c|  (P; 2^-25: f16's subnormals)
+      2^-8 |out|  (the output) + sum_c max(2^-11 p'_c, 2^-32 p'_top) |vcode_c|
+      (P: 2^-11 of a normal f16, 2^-25 of a subnormal one, the largest weight being held at 2^7 or above)
       + eps * sum_c p_c |v_c|,  eps = the scores' and the sums' fp32 rounding."""
     batch, tokens, q_heads, dim = query.shape
     kv_heads, capacity = cache["keys"].shape[1:3]
@@ -78,7 +79,7 @@ def attention(query, cache, position, scale, chain=None):
             size = torch.einsum("hgc,hcd->hgd", p, v.abs())
             weight = p * vs[:, None]
             top = weight.amax(-1, keepdim=True).clamp_min(1e-300)
-            rounding = torch.maximum(2.0 ** -11 * weight, 2.0 ** -25 * top)
+            rounding = torch.maximum(2.0 ** -11 * weight, 2.0 ** -32 * (1 + 2.0 ** -16) * top)  # 2^7 to fp32's rounding
             by_p = torch.einsum("hgc,hcd->hgd", rounding, codes.abs())
             largest = torch.einsum("hgd,hcd->hgc", q.abs(), k.abs()).amax() * abs(scale)
             eps = float(largest) * 4 * dim * 2.0 ** -23 + (len(at) / 16 + 64) * 2.0 ** -23 + 2.0 ** -20
