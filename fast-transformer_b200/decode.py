@@ -78,6 +78,12 @@ class QuantKVCache:
         """One row of one layer, as a cache of its own."""
         return QuantCache(*(t[i, layer, row:row + 1] for t in (self.store, self.scales) for i in range(2)), self.block)
 
+    def block_views(self, slot):
+        """The codes and scales of the block that holds ``slot``, every layer's: all that an append there
+        can change."""
+        at = slot // self.block
+        return self.store[..., at * self.block:(at + 1) * self.block, :].view(torch.uint8), self.scales[..., at]
+
     def nbytes_valid(self, length):
         """K+V bytes of all layers (codes and scales) for ``length`` valid slots per row."""
         _, layers, batch, kv_heads, _, dim = self.store.shape
@@ -361,12 +367,16 @@ class DecodeState:
     def capture(self, warmup=3):
         """Warm every kernel and shape choice eagerly on a side stream, then capture one step.
         The warmup steps write the slot at `position`, which every real step rewrites before
-        reading it."""
+        reading it. In an 8-bit cache they may also raise its block's scale and round the block's
+        earlier codes to it, which a later step cannot undo: the block is put back."""
         current = torch.cuda.current_stream(self.device)
         side = torch.cuda.Stream(device=self.device)
         # the copies are enqueued on the current stream before the side stream starts waiting
         # for it: the warm-up steps below run on the side stream and overwrite the originals
         saved_position, saved_tokens = self.position.clone(), self.token_ids.clone()
+        slot = int(self.position) if self.quantised else -1
+        block = self.cache.block_views(slot) if 0 <= slot < self.capacity else ()
+        saved_block = [part.clone() for part in block]
         side.wait_stream(current)
         with torch.cuda.stream(side):
             for _ in range(warmup):
@@ -377,6 +387,9 @@ class DecodeState:
         torch.cuda.synchronize(self.device)
         self.position.copy_(saved_position)
         self.token_ids.copy_(saved_tokens)
+        for part, saved in zip(block, saved_block):
+            part.copy_(saved)
+        del block, saved_block
         if self.peers is not None:
             self.peers.reset()  # the warmup pushed words flagged with the position replayed next
         self.graph = torch.cuda.CUDAGraph()
