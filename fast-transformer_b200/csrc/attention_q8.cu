@@ -22,7 +22,7 @@
 // a producer warp (one lane issues a TMA load per K and V tile, 16 lanes copy the tile's scales
 // with cp.async; both complete on the stage's mbarrier) and consumer warps; two CTAs share an SM: one
 // streams while the other starts or ends. S^T[16 x 8 NG] = K Q^T, a lazy pivot (it moves only when a
-// score passes it by more than 8, one vote), O^T += V^T P^T.
+// score passes it by kSlack, one vote), O^T += V^T P^T.
 //  * One column group: four consumers of two 16-slot slices each, whole in registers; a warp needs no
 //    other until the end.
 //  * More: the conversions and products of a tile, not its bytes, fill its time, and O^T of every warp
@@ -56,8 +56,9 @@ constexpr int kThreads = (kConsumers<NG> + 1) * 32;
 constexpr int kMaxBatch = 1024;
 constexpr int kScales = 2 * kSlices;  // per stage: K and V scale of each 16-slot slice
 constexpr int kMaxCluster = 16;      // above 8: the non-portable cluster size attribute
-constexpr float kSlack = 8.f;        // log2 a score may pass the pivot by before it moves
-constexpr float kLift = 7.f;         // log2 of the largest p' when its pivot moves: p' <= 2^(kLift + kSlack), f16 ends at 65504
+constexpr float kLift = 7.f;         // log2 of the largest p' when its pivot moves
+constexpr float kSlack = 15.f;       // log2 of p' or p at which the pivots move: f16 ends at 65504 (p stays in fp32; a test
+                                     // of its own against less cost 2 us of 27 with 20 members)
 
 struct Params {
   const __nv_bfloat16* q;  // [B, T, Hq, D]
@@ -413,7 +414,7 @@ __device__ __forceinline__ void attend_tile(State<D, 1>& a, const Params& p, con
 #pragma unroll
     for (int x = 0; x < H; ++x) {
       const float over = fmaxf(s[x][e], s[x][e + 2]) - a.m[0][e];
-      moves = moves || over > kSlack || over + lv[x] - a.r[0][e] > kLift + kSlack;
+      moves = moves || fmaxf(over, over + lv[x] - a.r[0][e]) > kSlack;
     }
   if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
@@ -547,10 +548,10 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
   // Weights on the pivots so far: one barrier a tile, unless they have to move, as in a run's first tile. They
   // move once at most: they are worked out with the same roundings as x and y, which are monotone, so that no x is
   // above 0 then and no y above 8, kLift rounded to a step of at most 8 (where steps are 16 and more it rounds to
-  // 0). A product fused into x would break that where scores round by more than 8.
+  // 0). A product fused into x would break that where scores round by more than kSlack.
   for (;; fresh = false) {
     if (!fresh) {
-      float top = 0.f, top_y = 0.f;
+      float top = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float x[4], y[4];  // s - m and s - m + log2 vs - r
@@ -565,17 +566,14 @@ __device__ __forceinline__ void attend_tile(State<D, NG>& a, const Params& p, co
             if (hidden >> (n * 4 + e) & 1) x[e] = y[e] = -INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          top = fmaxf(top, x[e]);
-          top_y = fmaxf(top_y, y[e]);
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(x[e], y[e]));
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
         weights[n * 64] = make_uint2(movmatrix_trans(pack_f16x2(y[0], y[1])), movmatrix_trans(pack_f16x2(y[2], y[3])));
         l[n][0] = ex2(x[0]) + ex2(x[2]);
         l[n][1] = ex2(x[1]) + ex2(x[3]);
       }
-      if (!consumers_any<NG>((top > kSlack || top_y > kLift + kSlack) && sm.misc[4 + warp] != k + 1)) break;
+      if (!consumers_any<NG>(top > kSlack && sm.misc[4 + warp] != k + 1)) break;
     }
     if (lane == 0) sm.misc[4 + warp] = k + 1;  // once a tile, whatever the scores
     __syncwarp();
