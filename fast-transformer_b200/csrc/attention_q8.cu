@@ -1365,7 +1365,14 @@ using namespace fb;
 extern "C" size_t fb_attention_q8_workspace(const fb_q8_cache* cache, int tokens, int q_heads) {
   attn8::Params p;
   if (cache == nullptr || attn8::shape(&p, *cache, tokens, q_heads) != FB_OK) return ~size_t(0);
-  return attn8::plan(p, cache->head_dim) > 0 ? 0 : attn8::workspace_bytes(p, cache->head_dim);
+  int devices = 0;
+  if (cudaGetDeviceCount(&devices) != cudaSuccess || devices == 0) {
+    cudaGetLastError();  // a host that sizes memory without a device: the most any form takes
+    return attn8::workspace_bytes(p, cache->head_dim);
+  }
+  const int cluster = attn8::plan(p, cache->head_dim);
+  if (cluster < 0) return ~size_t(0);  // the launch would fail too: no size to keep
+  return cluster > 0 ? 0 : attn8::workspace_bytes(p, cache->head_dim);
 }
 
 extern "C" int fb_attention_q8(const void* q, const fb_q8_cache* cache, const int64_t* position, int per_row,

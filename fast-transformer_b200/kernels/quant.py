@@ -84,7 +84,8 @@ class QuantCache:
                 need = int(lib.fb_attention_q8_workspace(self.address, tokens, q_heads))
             if need == ctypes.c_size_t(-1).value:
                 raise ValueError(f"8-bit attention of {tokens} x {q_heads} queries over a cache of {self.batch} x "
-                                 f"{self.kv_heads} x {self.capacity} slots is not supported")
+                                 f"{self.kv_heads} x {self.capacity} slots is not supported, or {self.device} refuses "
+                                 "its kernels")
             self._workspace[key] = need
         return need
 

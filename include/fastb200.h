@@ -208,8 +208,9 @@ int fb_spec_relocate_q8(void* store, float* scales, int planes, int batch, int k
  * fb_verify_attention).
  *   q   bf16 [B, T, Hq, D], 8-byte aligned; out bf16 [B, T, Hq, D]; any Hq / Hkv
  *   workspace: fb_attention_q8_workspace() bytes (it reads the cache's sizes, not its pointers; 0:
- *   the shape runs without, workspace may be NULL; (size_t)-1: the shape is not supported), 16-byte
- *   aligned, any contents; calls that overlap on the GPU need one each.
+ *   the shape runs without, workspace may be NULL; (size_t)-1: the shape is not supported, or the
+ *   current device refuses its kernels; without any device: what the shape takes at most on one of
+ *   148 SMs), 16-byte aligned, any contents; calls that overlap on the GPU need one each.
  *   B <= 1024, B * Hkv * C < 2^31.
  * fp32 scores, sums and accumulation; P in f16 for the value product. Everything is read after
  * the dependency wait: any kernel may have written the cache or the position just before. */

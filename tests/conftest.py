@@ -11,3 +11,5 @@ for path in (ROOT, PACKAGE, GOLDEN):
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA (B200) device; run with -m gpu")
+    if config.getoption("markexpr", "") == "not gpu":
+        os.environ["CUDA_VISIBLE_DEVICES"] = ""  # the same run on every machine: without a device

@@ -1,0 +1,30 @@
+"""Sizes and refusals of the quantised decode operators that need no GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+p = ctypes.c_void_p(1 << 20)  # never dereferenced
+NULL = None
+NO_DEVICE = not torch.cuda.is_available()
+
+
+def cache(batch=1, kv_heads=2, capacity=64, dim=128, block=64):
+    from kernels._native import Q8Cache
+    return Q8Cache(1 << 20, 1 << 20, 1 << 20, 1 << 20, batch, kv_heads, capacity, dim, block)
+
+
+@pytest.mark.skipif(not NO_DEVICE, reason="sizes of a host without a device")
+@pytest.mark.parametrize("batch,kv_heads,q_heads,tokens,dim", [(1, 2, 16, 1, 128), (64, 8, 16, 1, 128), (3, 2, 14, 5, 64),
+                                                              (2, 1, 36, 1, 64)])
+def test_attention_workspace_without_a_device(batch, kv_heads, q_heads, tokens, dim):
+    """The most any form takes: fp32 partials and four statistics for each of 296 CTAs and each unit."""
+    from kernels._native import lib
+    members = tokens * (q_heads // kv_heads)
+    chunks = -(-members // 32)
+    width = -(-members // chunks)
+    slots = 2 * 148 + batch * kv_heads * chunks
+    acc = -(-slots * width * dim * 4 // 256) * 256
+    c = cache(batch, kv_heads, 2048, dim)
+    assert lib.fb_attention_q8_workspace(ctypes.byref(c), tokens, q_heads) == acc + slots * width * 16

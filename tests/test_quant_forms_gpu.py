@@ -69,3 +69,18 @@ def test_small_weights_beside_a_leader(sliced, tokens, groups, dim):
     else:
         out = block_attention_q8(query.to(DEV), c, position.to(DEV), scale, chain.to(DEV))
     check(out, expect, bound)
+
+
+@pytest.mark.parametrize("batch,kv_heads,capacity,tokens,q_heads,sliced", [
+    (64, 8, 2048, 1, 16, False), (64, 8, 32768, 1, 16, True), (8, 8, 32768, 5, 32, False), (20, 8, LONG, 1, 32, True),
+    (1, 2, 64, 1, 16, False)])
+def test_workspace_says_which_form(batch, kv_heads, capacity, tokens, q_heads, sliced):
+    """Units of short rows, and up to one a SM, run as clusters without a workspace; the others take partials of
+    two CTAs an SM."""
+    import ctypes
+    from kernels._native import Q8Cache, lib
+    c = Q8Cache(1 << 20, 1 << 20, 1 << 20, 1 << 20, batch, kv_heads, capacity, 128, 64)  # sizes only
+    need = lib.fb_attention_q8_workspace(ctypes.byref(c), tokens, q_heads)
+    slots = 2 * torch.cuda.get_device_properties(0).multi_processor_count + batch * kv_heads
+    width = tokens * (q_heads // kv_heads)
+    assert need == (-(-slots * width * 128 * 4 // 256) * 256 + slots * width * 16 if sliced else 0)
