@@ -84,3 +84,185 @@ def test_workspace_says_which_form(batch, kv_heads, capacity, tokens, q_heads, s
     slots = 2 * torch.cuda.get_device_properties(0).multi_processor_count + batch * kv_heads
     width = tokens * (q_heads // kv_heads)
     assert need == (-(-slots * width * 128 * 4 // 256) * 256 + slots * width * 16 if sliced else 0)
+
+
+# ------------------------------------------------------------------ the grid of slices and its merge
+def stretched(cache, position, tokens, capacity=LONG):
+    """The cache at a larger capacity, NaN codes and scales in every slot behind each row's last token."""
+    out = {"block": cache["block"]}
+    block, short = cache["block"], cache["keys"].shape[2]
+    for name in ("key", "value"):
+        batch, heads, _, dim = cache[name + "s"].shape
+        codes = torch.full((batch, heads, capacity, dim), 0x7f, dtype=torch.uint8)
+        scales = torch.full((batch, heads, -(-capacity // block)), float("nan"))
+        for b in range(batch):
+            p = int(position[b if len(position) > 1 else 0])
+            end = 0 if p < 0 else min(p + tokens, short)
+            codes[b, :, :end] = cache[name + "s"].view(torch.uint8)[b, :, :end]
+            scales[b, :, :-(-end // block)] = cache[name + "_scales"][b, :, :-(-end // block)]
+        out[name + "s"], out[name + "_scales"] = codes.view(oq.E4M3), scales
+    return out
+
+
+def sliced_handle(cache, position, tokens, q_heads):
+    c = handle(stretched(cache, position, tokens))
+    assert c.workspace_bytes(tokens, q_heads) > 0  # the form these tests are about
+    return c
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens,q_heads", [(1, 32), (1, 72), (3, 32), (2, 80), (5, 40), (4, 64), (6, 48)])
+def test_slices_of_ragged_rows(tokens, q_heads, dim):
+    """One to four column groups (and two member groups), rows from empty to six tiles: slices end inside units
+    and cross them."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(100 * tokens + dim + q_heads)
+    batch, kv_heads, capacity = 20, 8, 700
+    position = torch.randint(-1, capacity - tokens + 1, (batch,), generator=g)
+    position[:4] = torch.tensor([-1, 0, capacity - tokens, 127])
+    chain = torch.randint(1, tokens + 1, (batch,), generator=g)
+    cache = oq.random_cache(batch, kv_heads, capacity, dim, 32, g)
+    query = torch.randn(batch, tokens, q_heads, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, cache, position, 1 / math.sqrt(dim), chain)
+    c = sliced_handle(cache, position, tokens, q_heads)
+    out = block_attention_q8(query.to(DEV), c, position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV))
+    check(out, expect, bound)
+    assert (out[0] == 0).all()
+    again = block_attention_q8(query.to(DEV), c, position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV))
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dim,q_heads", [(64, 16), (128, 96)])
+@pytest.mark.parametrize("lengths", [{}, {3: 1}, {0: 128}, {19: 129, 7: 16}, {2: 300, 11: 1, 12: 40}])
+def test_slices_fewer_than_ctas(lengths, dim, q_heads):
+    """Fewer tiles than CTAs, down to none: most slices are empty, and every row without a slot gives zeros."""
+    from kernels.decode_attention import decode_attention_q8
+    g = torch.Generator().manual_seed(dim + len(lengths))
+    batch, kv_heads = 20, 8
+    position = torch.full((batch,), -1)
+    for b, n in lengths.items():
+        position[b] = n - 1
+    cache = oq.random_cache(batch, kv_heads, 320, dim, 16, g)
+    query = torch.randn(batch, q_heads, 1, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query.transpose(1, 2), cache, position, 0.1)
+    c = sliced_handle(cache, position, 1, q_heads)
+    out = decode_attention_q8(query.to(DEV), c, position.to(DEV), 0.1)
+    check(out, expect, bound)
+    assert (out[position.to(DEV) < 0] == 0).all()
+
+
+@pytest.mark.parametrize("position", [-1, 0, 128, 611])
+def test_slices_at_a_shared_position(position):
+    from kernels.decode_attention import decode_attention_q8
+    g = torch.Generator().manual_seed(position + 2)
+    batch, kv_heads, dim, position = 20, 8, 128, torch.tensor([position])
+    cache = oq.random_cache(batch, kv_heads, 640, dim, 64, g)
+    query = torch.randn(batch, 32, 1, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query.transpose(1, 2), cache, position, 0.09)
+    c = sliced_handle(cache, position, 1, 32)
+    check(decode_attention_q8(query.to(DEV), c, position.to(DEV), 0.09), expect, bound)
+
+
+@pytest.mark.parametrize("tokens,dim", [(1, 128), (1, 64), (3, 128), (4, 64), (5, 64), (7, 128)])
+def test_slices_of_rising_scores_and_uneven_scales(tokens, dim):
+    """Scores that rise from block to block, so that the pivots move in every tile and differ between the runs
+    that are merged, and value scales 2^40 apart, 2^-100 or 0, so that the value product's pivot moves on its
+    own."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(dim + tokens)
+    batch, capacity, kv_heads = 40, 800, 4
+    cache = oq.random_cache(batch, kv_heads, capacity, dim, 64, g)
+    blocks = cache["key_scales"].shape[2]
+    cache["key_scales"] *= torch.exp2(torch.linspace(-2, 3, blocks).round())
+    cache["value_scales"][0] = torch.exp2(torch.linspace(-30, 10, blocks).round())
+    cache["value_scales"][1] = torch.exp2(torch.linspace(10, -30, blocks).round())
+    cache["value_scales"][1, :, ::3] = 0.0
+    cache["value_scales"][2] = 0.0
+    cache["values"][3] = torch.zeros(kv_heads, capacity, dim).to(oq.E4M3)
+    cache["value_scales"][3] = 2.0 ** -100
+    cache["value_scales"][4] *= 1.37
+    cache["key_scales"][4] *= 0.81
+    position = torch.full((batch,), capacity - tokens)
+    position[5:] = torch.randint(400, capacity - tokens + 1, (batch - 5,), generator=g)
+    chain = torch.full((batch,), tokens)
+    query = torch.randn(batch, tokens, kv_heads * 4, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, cache, position, 1 / math.sqrt(dim), chain)
+    c = sliced_handle(cache, position, tokens, kv_heads * 4)
+    out = block_attention_q8(query.to(DEV), c, position.to(DEV), 1 / math.sqrt(dim), chain.to(DEV))
+    check(out, expect, bound + 1e-40)
+
+
+@pytest.mark.parametrize("tokens,dim", [(2, 128), (4, 64), (4, 128), (8, 128)])
+def test_slices_hide_nan_of_the_last_draft(tokens, dim):
+    """A NaN in the last draft's slot stays with the token that sees it, where slices end inside the rows."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(tokens + dim)
+    batch, capacity = 24, 300
+    position = torch.randint(0, capacity - tokens + 1, (batch,), generator=g)
+    chain = torch.full((batch,), tokens)
+    sound = oq.random_cache(batch, 8, capacity, dim, 16, g)
+    cache = {k: v.clone() if torch.is_tensor(v) else v for k, v in sound.items()}
+    for b in range(batch):
+        cache["values"].view(torch.uint8)[b, :, int(position[b]) + tokens - 1, 9] = 0xff
+    query = torch.randn(batch, tokens, 32, dim, generator=g).bfloat16()
+    expect, bound = oq.attention(query, sound, position, 0.1, chain)
+    c = sliced_handle(cache, position, tokens, 32)
+    out = block_attention_q8(query.to(DEV), c, position.to(DEV), 0.1, chain.to(DEV)).cpu()
+    assert torch.isnan(out[:, -1, :, 9]).all()
+    hidden = torch.ones_like(out, dtype=torch.bool)
+    hidden[:, -1, :, 9] = False
+    assert torch.isfinite(out[hidden]).all()
+    assert ((out.double() - expect).abs()[hidden] <= bound[hidden]).all()
+
+
+def sliced_jobs(g):
+    """Two calls' inputs over caches whose attention takes partials."""
+    from kernels.decode_attention import block_attention_q8, decode_attention_q8
+    jobs = []
+    for _ in range(2):
+        position = torch.randint(0, 595, (24,), generator=g)
+        c = sliced_handle(oq.random_cache(24, 8, 600, 128, 64, g), position, 5, 32)
+        assert c.workspace_bytes(1, 32) > 0
+        q = torch.randn(24, 5, 32, 128, generator=g).bfloat16().to(DEV)
+        one, chain, at = q[:, :1].transpose(1, 2).contiguous(), torch.full((24,), 5).to(DEV), position.to(DEV)
+        jobs.append(lambda c=c, q=q, one=one, chain=chain, at=at: (decode_attention_q8(one, c, at, 0.09),
+                                                                   block_attention_q8(q, c, at, 0.09, chain)))
+    return jobs
+
+
+def test_slices_on_two_streams_at_once():
+    """Calls that overlap on the GPU share no partials: the results are those of calls in turn."""
+    jobs = sliced_jobs(torch.Generator().manual_seed(31))
+    expect = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], [[], []]
+    for _ in range(20):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(job())
+    torch.cuda.synchronize()
+    for want, runs in zip(expect, got):
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(want, run))
+
+
+def test_slices_of_two_graphs_and_eager_calls():
+    """Two graphs on one cache handle, replayed on two streams at once beside eager calls on it."""
+    job, other = sliced_jobs(torch.Generator().manual_seed(32))
+    expect, beside = job(), other()
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for stream in streams:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(job())
+        graphs.append(graph)
+    eager = []
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager.append((job(), other()))
+    torch.cuda.synchronize()
+    for got, want in (*((o, expect) for o in outs), *((e, expect) for e, _ in eager), *((e, beside) for _, e in eager)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
