@@ -532,6 +532,7 @@ extern "C" int fb_spec_relocate_q8(void* store, float* scales, int planes, int b
   if (!store || !scales || !move_from || !move_to || planes <= 0 || batch <= 0 || kv_heads <= 0 || capacity <= 0)
     return FB_ERR_ARG;
   if ((head_dim != 64 && head_dim != 128) || !q8::valid_block(block)) return FB_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(store) & 3u) return FB_ERR_ARG;  // codes move four at a time
   const long long warps = static_cast<long long>(planes) * batch * kv_heads;
   if ((warps + 3) / 4 >= (1ll << 31)) return FB_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>((warps + 3) / 4)), threads(128);

@@ -576,6 +576,7 @@ extern "C" int fb_w4_pack(const int8_t* codes, const void* scales, void* packed,
                           void* stream) {
   if (!codes || !scales || !packed) return FB_ERR_ARG;
   if (!w4::valid(n, k, group)) return FB_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(packed) & 15u) return FB_ERR_ARG;
   return launch_ex(w4::pack_kernel, dim3(sm_count() * 8), dim3(256), 0, static_cast<cudaStream_t>(stream), 1, codes,
                    static_cast<const __nv_bfloat16*>(scales), static_cast<uint8_t*>(packed), n,
                    w4::layout_of(n, k, group));
@@ -584,6 +585,7 @@ extern "C" int fb_w4_pack(const int8_t* codes, const void* scales, void* packed,
 extern "C" int fb_w4_dequantize(const void* packed, void* out, int n, int k, int group, void* stream) {
   if (!packed || !out) return FB_ERR_ARG;
   if (!w4::valid(n, k, group)) return FB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(packed) | reinterpret_cast<uintptr_t>(out)) & 15u) return FB_ERR_ARG;
   return launch_ex(w4::dequantize_kernel, dim3(sm_count() * 8), dim3(256), 0, static_cast<cudaStream_t>(stream), 1,
                    static_cast<const uint8_t*>(packed), static_cast<__nv_bfloat16*>(out), n, w4::layout_of(n, k, group));
 }

@@ -184,7 +184,8 @@ int fb_qk_norm_rope_append(const void* packed, int packed_splits, const void* q_
  *   behind the last token keep their codes. Slots past C and table phases outside [0, C) set the
  *   error word (the store is skipped, the phase clamped).
  * fb_spec_relocate_q8: fb_spec_relocate for a store [planes, B, Hkv, C, D] with scales [planes, B,
- *   Hkv, ceil(C / block)]: move_to becomes its block's newest slot, by the append's rule.
+ *   Hkv, ceil(C / block)]: move_to becomes its block's newest slot, by the append's rule. The store is
+ *   4-byte aligned.
  * ---------------------------------------------------------------------------------- */
 typedef struct fb_q8_cache {
   void* keys;
@@ -230,7 +231,8 @@ int fb_attention_q8(const void* q, const fb_q8_cache* cache, const int64_t* posi
  *   gate/up blocks as for fb_linear (N % 128 == 0): out bf16 [M, N / 2].
  *   The packed weights may be read before the wait on the previous kernel, like
  *   fb_linear's: that kernel must not write them.
- * fb_w4_dequantize: the weights as bf16 [N, K] (code * scale rounded once), for library products.
+ * fb_w4_dequantize: the weights as bf16 [N, K] (code * scale rounded once; out 16-byte aligned), for
+ *   library products.
  * ---------------------------------------------------------------------------------- */
 size_t fb_w4_packed_bytes(int n, int k, int group);
 int fb_w4_pack(const int8_t* codes, const void* scales, void* packed, int n, int k, int group,

@@ -15,6 +15,21 @@ def cache(batch=1, kv_heads=2, capacity=64, dim=128, block=64):
     return Q8Cache(1 << 20, 1 << 20, 1 << 20, 1 << 20, batch, kv_heads, capacity, dim, block)
 
 
+def test_misaligned_pointers_are_refused():
+    """Codes can lie at any byte; the kernels read and write them (and what they expand to) in wider words."""
+    from kernels._native import lib
+
+    def at(offset):
+        return ctypes.c_void_p((1 << 20) + offset)
+
+    for offset in (1, 2, 3):
+        assert lib.fb_spec_relocate_q8(at(offset), p, 4, 2, 2, 64, 128, 64, p, p, NULL) == -1
+    for offset in (1, 2, 4, 8):
+        assert lib.fb_w4_pack(p, p, at(offset), 8, 32, 32, NULL) == -1
+        assert lib.fb_w4_dequantize(at(offset), p, 8, 32, 32, NULL) == -1
+        assert lib.fb_w4_dequantize(p, at(offset), 8, 32, 32, NULL) == -1
+
+
 @pytest.mark.skipif(not NO_DEVICE, reason="sizes of a host without a device")
 @pytest.mark.parametrize("batch,kv_heads,q_heads,tokens,dim", [(1, 2, 16, 1, 128), (64, 8, 16, 1, 128), (3, 2, 14, 5, 64),
                                                               (2, 1, 36, 1, 64)])
