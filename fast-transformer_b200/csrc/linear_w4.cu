@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* packed, 
 
 bool valid(int n, int k, int group) {
   return n > 0 && k > 0 && n % 8 == 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 &&
-         n < (1 << 23) && k < (1 << 27);
+         n < (1 << 23) && k < (1 << 27) && static_cast<long long>(n) * k <= 1ll << 34;  // Word's 32-bit row count
 }
 
 Layout layout_of(int n, int k, int group) {

@@ -223,7 +223,7 @@ int fb_attention_q8(const void* q, const fb_q8_cache* cache, const int64_t* posi
 /* ------------------------------------------------------------------------------------
  * Projections with 4-bit weights (no counterpart in the reference): y = x @ W^T,
  * W[n, k] = code[n, k] * scale[n, k / group], codes -8..7, group in {32, 64, 128}, K % group == 0,
- * N % 8 == 0.
+ * N % 8 == 0, N * K <= 2^34.
  * fb_w4_pack lays codes int8 [N, K] and scales bf16 [N, K / group] out once, into packed
  *   (fb_w4_packed_bytes(), 16-byte aligned); codes outside -8..7 keep their low four bits.
  * fb_linear_w4: x bf16 [M, K] (M <= 64, 16-byte aligned); fp32 accumulation of the exact products, one rounding.

@@ -43,3 +43,14 @@ def test_attention_workspace_without_a_device(batch, kv_heads, q_heads, tokens, 
     acc = -(-slots * width * dim * 4 // 256) * 256
     c = cache(batch, kv_heads, 2048, dim)
     assert lib.fb_attention_q8_workspace(ctypes.byref(c), tokens, q_heads) == acc + slots * width * 16
+
+
+def test_weights_past_the_layouts_index_range_are_refused():
+    """The layout's kernels count rows of codes in 32 bits: at most 2^34 weights."""
+    from kernels._native import lib
+    assert lib.fb_w4_packed_bytes(1 << 20, 1 << 14, 128) == (1 << 33) + (1 << 20) * (1 << 7) * 2
+    for n, k in ((1 << 20, (1 << 14) + 128), (1 << 22, 1 << 14), (1 << 22, 1 << 20)):
+        assert lib.fb_w4_packed_bytes(n, k, 128) == 0
+        assert lib.fb_w4_pack(p, p, p, n, k, 128, NULL) == -2
+        assert lib.fb_w4_dequantize(p, p, n, k, 128, NULL) == -2
+        assert lib.fb_linear_w4(p, p, p, 1, n, k, 128, 0, NULL) == -2
