@@ -65,6 +65,7 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, cache, q_heads,
     tokens = shape[1]
     assert data.dtype == (torch.float32 if split else torch.bfloat16) and data.is_contiguous()
     assert shape == (batch, tokens, (q_heads + 2 * kv_heads) * dim) and q_heads > 0
+    assert not split or splits > 0 and data.shape == (splits, batch * tokens, shape[2])
     assert 0 < tokens <= capacity
     assert not (rows and prefill) and not (table and (rows or prefill))
     if phases is not None:

@@ -54,3 +54,18 @@ def test_weights_past_the_layouts_index_range_are_refused():
         assert lib.fb_w4_pack(p, p, p, n, k, 128, NULL) == -2
         assert lib.fb_w4_dequantize(p, p, n, k, 128, NULL) == -2
         assert lib.fb_linear_w4(p, p, p, 1, n, k, 128, 0, NULL) == -2
+
+
+@pytest.mark.parametrize("partial", [(0, 3, 1024), (2, 2, 1024), (2, 3, 1023), (3, 1024)])
+def test_append_refuses_partials_that_are_not_its_shape(partial):
+    """A Split carries its logical shape beside its buffer: the two have to agree before a kernel reads by the
+    first."""
+    from types import SimpleNamespace
+    from kernels.merged import Split
+    from kernels.qk_rope import qk_rope_cache_q8
+    c = SimpleNamespace(batch=3, kv_heads=2, capacity=40, dim=128, device=torch.device("cuda", 0), block=16)
+    norm = SimpleNamespace(weight=torch.ones(128, dtype=torch.bfloat16), variance_epsilon=1e-6)
+    phase = torch.zeros(1, 1, 128, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError):
+        qk_rope_cache_q8(Split(torch.zeros(partial), (3, 1, 1024)), norm, norm, phase, phase,
+                         torch.zeros(1, dtype=torch.int64), c, 4)
