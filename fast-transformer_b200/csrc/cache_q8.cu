@@ -58,10 +58,12 @@ struct AppendParams {
   unsigned* err;
 };
 
-// Slot of a row's first token; negative: the row holds no sequence (nothing is appended).
+// Slot of a row's first token; negative: the row holds no sequence (nothing is appended). Held where a token's
+// offset cannot carry it past 64 bits; anything from the capacity on is past the cache alike.
+constexpr long long kFar = 1ll << 61;
 __device__ __forceinline__ long long first_slot(const AppendParams& p, int b) {
   if (p.mode == 1) return 0;
-  return p.position[p.mode == 2 ? b : 0];
+  return min(static_cast<long long>(p.position[p.mode == 2 ? b : 0]), kFar);
 }
 
 // The cos/sin row of token t of row b. Whole tables have at least `capacity` rows: a phase
@@ -69,7 +71,9 @@ __device__ __forceinline__ long long first_slot(const AppendParams& p, int b) {
 __device__ __forceinline__ long long phase_row(const AppendParams& p, int b, int t, long long start) {
   const int row = b * p.tokens + t;
   if (!p.table) return p.mode == 2 ? row : t;
-  long long phase = start + (p.phases != nullptr ? p.phases[row] : t);
+  long long offset = p.phases != nullptr ? p.phases[row] : t;
+  offset = max(-kFar, min(offset, kFar));
+  long long phase = max(-kFar, start) + offset;
   if (phase < 0 || phase >= p.capacity) {
     if (start >= 0) raise_error(p.err, kErrBadShape);
     phase = phase < 0 ? 0 : p.capacity - 1;
@@ -297,11 +301,15 @@ __global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_k
   const int pair = item >> 1;
   const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
   const long long start = first_slot(p, b);
-  if (start < 0) return;  // whole CTA
+  if (start < 0 || start >= p.capacity) {  // whole CTA: an empty row, or every token past the cache
+    if (start >= 0 && threadIdx.x == 0) raise_error(p.err, kErrBadShape);
+    return;
+  }
   const long long at = (start >> p.block_shift) + nth;  // block index
   const long long low = at << p.block_shift;
-  if (low >= p.capacity || low >= start + p.tokens) {
-    if (low < start + p.tokens && threadIdx.x == 0) raise_error(p.err, kErrBadShape);  // tokens past the cache
+  if (low >= start + p.tokens) return;
+  if (low >= p.capacity) {
+    if (threadIdx.x == 0) raise_error(p.err, kErrBadShape);  // tokens past the cache
     return;
   }
   uint8_t* codes = (is_value ? p.values : p.keys) + (static_cast<size_t>(pair) * p.capacity + low) * D + d0;

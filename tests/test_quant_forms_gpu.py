@@ -266,3 +266,50 @@ def test_slices_of_two_graphs_and_eager_calls():
     torch.cuda.synchronize()
     for got, want in (*((o, expect) for o in outs), *((e, expect) for e, _ in eager), *((e, beside) for _, e in eager)):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------ append
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("start", [70, 79, 80, 2 ** 61, 2 ** 62, 2 ** 63 - 70, 2 ** 63 - 2, 2 ** 63 - 1])
+def test_append_past_the_cache_writes_nothing(start, tokens):
+    """From the first slot past the cache (in its last block, whose scale is 0 here) to positions whose sum with
+    the token count leaves 64 bits: neither codes nor scales change, the error word is set, and the queries are
+    those of the same phases."""
+    from types import SimpleNamespace
+    from kernels import _native
+    from kernels.qk_rope import qk_rope_cache_q8
+    g = torch.Generator().manual_seed(tokens)
+    cache = oq.random_cache(1, 1, 70, 64, 16, g)
+    cache["key_scales"][..., -1] = cache["value_scales"][..., -1] = 0
+    c = handle(cache)
+    norms = [SimpleNamespace(weight=torch.ones(64, dtype=torch.bfloat16, device=DEV), variance_epsilon=1e-6)] * 2
+    packed = torch.randn(1, tokens, 3 * 64, generator=g).bfloat16().to(DEV)
+    cos, sin = (torch.randn(1, tokens, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    out = qk_rope_cache_q8(packed, *norms, cos, sin, torch.tensor([start], device=DEV), c, 1)
+    assert _native.device_error() != 0
+    for name in ("keys", "values"):
+        assert torch.equal(getattr(c, name).cpu().view(torch.uint8), cache[name].view(torch.uint8))
+        assert torch.equal(getattr(c, name[:-1] + "_scales").cpu(), cache[name[:-1] + "_scales"])
+    assert torch.equal(out, qk_rope_cache_q8(packed, *norms, cos, sin, torch.tensor([0], device=DEV), c, 1))
+
+
+@pytest.mark.parametrize("phase", [-2 ** 63, -43, 30, 2 ** 63 - 1])
+def test_append_clamps_phases_outside_the_tables(phase):
+    """A phase that leaves the tables is reported and read at the nearest end, whatever it adds up to."""
+    from types import SimpleNamespace
+    from kernels import _native
+    from kernels.qk_rope import qk_rope_cache_q8
+    g = torch.Generator().manual_seed(3)
+    one, two = (oq.random_cache(2, 1, 70, 64, 16, torch.Generator().manual_seed(5)) for _ in range(2))
+    a, b = handle(one), handle(two)
+    norms = [SimpleNamespace(weight=torch.ones(64, dtype=torch.bfloat16, device=DEV), variance_epsilon=1e-6)] * 2
+    packed = torch.randn(2, 1, 4 * 64, generator=g).bfloat16().to(DEV)
+    cos, sin = (torch.randn(70, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    at = torch.tensor([41, 42], device=DEV)
+    nearest = torch.full((2, 1), 0 if phase < 0 else 69, device=DEV)
+    query = qk_rope_cache_q8(packed, *norms, cos, sin, at, a, 2, rows=True, phases=torch.full((2, 1), phase, device=DEV))
+    assert _native.device_error() != 0
+    expect = qk_rope_cache_q8(packed, *norms, cos, sin, at, b, 2, rows=True, phases=nearest - at[:, None])
+    assert torch.equal(query, expect)
+    for name in ("keys", "values"):
+        assert torch.equal(getattr(a, name).view(torch.uint8), getattr(b, name).view(torch.uint8))
