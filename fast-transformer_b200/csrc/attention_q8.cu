@@ -903,6 +903,12 @@ __device__ __forceinline__ int first_position(const Params& p, int b) {
   return static_cast<int>(min(p.position[p.per_row ? b : 0], static_cast<int64_t>(p.capacity)));
 }
 
+// Tokens of row b's chain: all of a longer one, none of a negative one.
+__device__ __forceinline__ int chain_of(const Params& p, int b) {
+  if (p.chain == nullptr) return 1;
+  return static_cast<int>(max(static_cast<int64_t>(0), min(p.chain[b], static_cast<int64_t>(p.tokens))));
+}
+
 // ------------------------------------------------------------------------------ cluster form
 template <int D, int NG>
 __global__ void __launch_bounds__(kThreads<NG>, 2)
@@ -932,7 +938,7 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
     return;
   }
   const int position = first_position(p, b);
-  const int chain = p.chain != nullptr ? static_cast<int>(p.chain[b]) : 1;
+  const int chain = chain_of(p, b);
   const int members = min(p.width, p.members - chunk * p.width);
   State<D, NG> a;
   start_unit<D, NG>(a, p, sm.query, b, h, chunk, warp, lane);
@@ -1091,7 +1097,7 @@ __global__ void __launch_bounds__(kThreads<NG>, 2)
       n = cum[b + 1] - cum[b];
       len = row_length(p, b);
       position = first_position(p, b);
-      if (p.chain != nullptr) chain = static_cast<int>(p.chain[b]);
+      chain = chain_of(p, b);
       run_first = j;
       start_unit<D, NG>(a, p, sm.query, b, u / p.chunks, u % p.chunks, warp, lane);
     }

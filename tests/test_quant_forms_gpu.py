@@ -313,3 +313,20 @@ def test_append_clamps_phases_outside_the_tables(phase):
     assert torch.equal(query, expect)
     for name in ("keys", "values"):
         assert torch.equal(getattr(a, name).view(torch.uint8), getattr(b, name).view(torch.uint8))
+
+
+@pytest.mark.parametrize("sliced", [False, True])
+def test_chains_longer_than_the_block(sliced):
+    """A chain of any length from the block's on is the whole block."""
+    from kernels.decode_attention import block_attention_q8
+    g = torch.Generator().manual_seed(17)
+    batch, kv_heads, tokens = (20, 8, 4) if sliced else (3, 2, 4)
+    position = torch.randint(0, 290, (batch,), generator=g)
+    cache = oq.random_cache(batch, kv_heads, 300, 64, 32, g)
+    query = torch.randn(batch, tokens, kv_heads * 2, 64, generator=g).bfloat16()
+    whole = torch.full((batch,), tokens)
+    expect, bound = oq.attention(query, cache, position, 0.125, whole)
+    c = sliced_handle(cache, position, tokens, kv_heads * 2) if sliced else handle(cache)
+    for length in (tokens, 7, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1):
+        out = block_attention_q8(query.to(DEV), c, position.to(DEV), 0.125, torch.full((batch,), length).to(DEV))
+        check(out, expect, bound)
