@@ -123,7 +123,7 @@ def _check_shape(n, k, group):
 
 def pack_weight4(codes, scales):
     """``Weight4`` of int8 codes [N, K] in -8..7 and bf16 scales [N, K / group] (weights are laid out
-    once, at load: the call checks the codes on the host and so synchronises)."""
+    once, at load: the call checks codes and scales on the host and so synchronises)."""
     if codes.dtype != torch.int8 or scales.dtype != torch.bfloat16 or codes.dim() != 2 or scales.dim() != 2:
         raise ValueError("4-bit weights are packed from int8 codes [N, K] and bf16 scales [N, K / group]")
     n, k = codes.shape
@@ -132,9 +132,11 @@ def pack_weight4(codes, scales):
     group = k // scales.shape[1]
     _check_shape(n, k, group)
     _native.require_device(codes.device, codes, scales)
-    low, high = torch.stack(torch.aminmax(codes)).tolist()
+    low, high, finite = torch.stack((*torch.aminmax(codes), torch.isfinite(scales).all().to(torch.int8))).tolist()
     if low < -8 or high > 7:
         raise ValueError("4-bit codes lie in -8..7")
+    if not finite:  # a product scales its groups' sums: 0 times infinity would not show
+        raise ValueError("4-bit weights take finite scales")
     codes, scales = codes.contiguous(), scales.contiguous()
     packed = torch.empty(int(lib.fb_w4_packed_bytes(n, k, group)), dtype=torch.uint8, device=codes.device)
     _native.launch("fb_w4_pack", codes.device, codes.data_ptr(), scales.data_ptr(), packed.data_ptr(), n, k, group)

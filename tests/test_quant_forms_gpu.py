@@ -330,3 +330,15 @@ def test_chains_longer_than_the_block(sliced):
     for length in (tokens, 7, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1):
         out = block_attention_q8(query.to(DEV), c, position.to(DEV), 0.125, torch.full((batch,), length).to(DEV))
         check(out, expect, bound)
+
+
+# ------------------------------------------------------------------------------ 4-bit weights
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_pack_weight4_refuses_scales_that_are_not_finite(bad):
+    from kernels.quant import pack_weight4
+    codes = torch.zeros(16, 128, dtype=torch.int8, device=DEV)
+    scales = torch.ones(16, 2, dtype=torch.bfloat16, device=DEV)
+    pack_weight4(codes, scales)
+    scales[11, 1] = bad
+    with pytest.raises(ValueError):
+        pack_weight4(codes, scales)
