@@ -342,3 +342,59 @@ def test_pack_weight4_refuses_scales_that_are_not_finite(bad):
     scales[11, 1] = bad
     with pytest.raises(ValueError):
         pack_weight4(codes, scales)
+
+
+# ------------------------------------------------------------------------------ far slots
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_offsets_past_32_bits(tokens):
+    """Codes past 2^32 bytes into the cache: an append at the last slots, attention over rows of 1.9 and 2.2
+    million slots whose keys are zero but for the appended ones and whose values are 1 / 128, and moves there and
+    back. Tolerance: the output's rounding, and of the sizes 2^-11 for P, 2^-11.5 for scores up to 45 summed over 128
+    dims in fp32, 2^-11.9 for 2200 fp32 sums a warp: below 2^-9 together."""
+    from types import SimpleNamespace
+    from kernels.decode_attention import block_attention_q8
+    from kernels.qk_rope import qk_rope_cache_q8
+    from kernels.quant import QuantCache
+    from kernels.spec import relocate_q8
+    batch, kv_heads, groups, dim, capacity, block = 2, 8, 2, 128, 2_200_003, 64
+    g = torch.Generator(device=DEV).manual_seed(6)
+    store = torch.zeros(2, 1, batch, kv_heads, capacity, dim, dtype=torch.uint8, device=DEV)
+    store[1].fill_(0x38)  # the code of 1
+    store = store.view(oq.E4M3)
+    scales = torch.full((2, 1, batch, kv_heads, -(-capacity // block)), 2.0 ** -7, device=DEV)
+    c = QuantCache(store[0, 0], store[1, 0], scales[0, 0], scales[1, 0], block)
+    assert c.keys.numel() > 2 ** 32
+    starts = [capacity - tokens, 1_900_001]
+    position = torch.tensor(starts, device=DEV)
+    packed = torch.randn(batch, tokens, (groups + 2) * kv_heads * dim, device=DEV, generator=g).bfloat16()
+    norm = SimpleNamespace(weight=torch.ones(dim, dtype=torch.bfloat16, device=DEV), variance_epsilon=1e-6)
+    cos, sin = (torch.full((batch, tokens, dim), v, device=DEV).bfloat16() for v in (1.0, 0.0))
+    query = qk_rope_cache_q8(packed, norm, norm, cos, sin, position, c, groups * kv_heads, rows=True).transpose(1, 2)
+    new = packed.view(batch, tokens, (groups + 2) * kv_heads, dim)[:, :, (groups + 1) * kv_heads:]
+    out = block_attention_q8(query, c, position, 1.0, torch.full((batch,), tokens, device=DEV))
+
+    def held(codes, scale, b, low, high):  # [Hkv, slots, D]: what slots of one block or two stand for
+        at = torch.arange(low, high, device=DEV)
+        return codes[b, :, low:high].double() * scale[b][:, at // block, None].double()
+
+    for b, low in enumerate(starts):
+        keys, values = (held(*x, b, low, low + tokens) for x in ((c.keys, c.key_scales), (c.values, c.value_scales)))
+        want = new[b].transpose(0, 1).double()
+        step = c.value_scales[b][:, torch.arange(low, low + tokens, device=DEV) // block, None].double()
+        assert ((values - want).abs() <= torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * step)).all()
+        assert (held(c.values, c.value_scales, b, low - 2, low) == 2.0 ** -7).all()
+        for t in range(tokens):
+            q = query[b, t].double().view(kv_heads, groups, dim)
+            p = torch.exp(torch.einsum("hgd,htd->hgt", q, keys[:, :t + 1]))
+            total = low + p.sum(-1, keepdim=True)
+            expect = (low * 2.0 ** -7 + torch.einsum("hgt,htd->hgd", p, values[:, :t + 1])) / total
+            size = (low * 2.0 ** -7 + torch.einsum("hgt,htd->hgd", p, values[:, :t + 1].abs())) / total
+            off = (out[b, t].double().view(kv_heads, groups, dim) - expect).abs()
+            assert (off <= 2.0 ** -8 * expect.abs() + 2.0 ** -9 * size).all(), (b, t)
+    c.values.view(torch.uint8)[1, :, capacity - 9] = 0x40  # 2
+    relocate_q8(store, scales, block, torch.tensor([40, capacity - 9], device=DEV),
+                torch.tensor([capacity - 1, 40], device=DEV))
+    assert (held(c.values, c.value_scales, 0, capacity - 1, capacity) == 2.0 ** -7).all()
+    assert (held(c.values, c.value_scales, 1, 40, 41) == 2.0 ** -6).all()
+    del store, c
+    torch.cuda.empty_cache()
