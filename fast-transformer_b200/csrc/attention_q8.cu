@@ -36,9 +36,10 @@
 //    (O, M, m, l) partials that a second launch merges in CTA order. No counters, no atomics:
 //    calls share nothing.
 // Measured (D = 128, blocks of 64): 16 rows x 8320 slots, 32 + 8 heads 45.4 us, 6.0 TB/s (0.92 of a copy's rate);
-// 64 rows of 1024 to 32768 slots 349 us, 6.3 TB/s; one row of 2048 slots 5.6 us, most of it launch, the chain
-// position - tile - product, and the merge; 8 rows x 4101 slots x 5 tokens 28.5 us, 2.4 TB/s: 0.36 of the issue
-// slots, the warps waiting on each other's weights, on conversions and on shared memory.
+// 64 rows of 1024 to 32768 slots 352 us, 6.3 TB/s; one row of 2048 slots 6.1 us (5.4 from L2), most of it launch, the
+// chain position - tile - product, all of it behind the dependency wait, and the merge; 8 rows x 4101 slots x 5
+// tokens 28 us, 2.4 TB/s: 0.36 of the issue slots, the warps waiting on each other's weights, on conversions and on
+// shared memory.
 #include <atomic>
 #include <type_traits>
 
@@ -1311,14 +1312,20 @@ int resident_clusters(int c) {
   return n;
 }
 
-// Tiles up to which a CTA per unit beats the persistent form's slices whatever the lengths: the merge and the
-// partials cost more than uneven rows. 64 rows of 8 KV heads: up to 4101 slots of any length 59 us against 92,
-// 4101 slots each 86 against 92; 24 rows of up to 8197 slots 58 against 47, of up to 32768 240 against 156.
+// Tiles of the cache up to which units past one an SM get a CTA each; beyond, the persistent form's slices, whose
+// merge and partials cost more than uneven rows do at few tiles. us, CTA per unit against slices, rows of 8 KV heads:
+// decode of 64 x 4101 slots 86 against 92 (lengths from an eighth on 63 against 70), 64 x 4608 93 against 102, 24 x 4101
+// 38 against 43 (34 against 33), and past the border 64 x 8197 159 against 172 (115 against 108), 24 x 8197 69 against 72
+// (63 against 50): even rows of any length would stay with a CTA each, ragged ones would not. Verify blocks of 5
+// tokens, 20 members: 20 x 2053 44 against 46, 32 x 4101 77 against 99, 64 x 4101 150 against 176, 20 x 8197 144 against
+// 110; the rule is wrong for 20 x 4101, whose 160 units leave most SMs with one of two CTAs: 77 against 68 (66 against 53).
 constexpr int kUnitTiles = 36;
 
 // The cluster size of a launch, 0 for the persistent form. Up to a unit per SM: the largest whose clusters are
-// all resident at once, no larger than the cache has tiles (64 units of 33 tiles, 20 members: 28 us, the
-// persistent form 43).
+// all resident at once, no larger than the cache has tiles. us by size (0: persistent): 64 units of 33 tiles, 20
+// members 0 43, 1 56, 2 33, 4 28 (taken), 8 36; 128 units of 65 tiles 0 54, 1 53, 2 45 (taken), 4 49; 8 units of 16 tiles 4
+// 7.0, 8 5.8, 16 6.1 (taken); 10 units of 8 tiles, D = 64, 4 5.1, 8 4.6 (taken); 16 units of 7 tiles, 32 members, D = 64
+// 4 9.7, 7 10.1 (taken). Near the top a size is within 0.4 of the next: the merge grows as the tiles shrink.
 template <int D, int NG>
 int cluster_size(const Params& p) {
   const int units = p.batch * p.kv_heads * p.chunks, tiles = tiles_of(p.capacity);

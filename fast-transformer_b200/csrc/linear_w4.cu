@@ -10,9 +10,9 @@
 // them back, multiplies by its scale in fp32 and adds them to its row's totals in registers. (A
 // first form with mma.sync spent twice the instructions on fragments, addends and scaling.)
 //
-// Measured (us, GB/s of codes and scales): 24576 x 4096, group 128, M = 16 19.9, 2.7 TB/s (without the
-// conversion about 15, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
-// merge); 4096 x 12288, group 32, M = 5 11.8, 2.4 TB/s; 6144 x 4096, M = 64 12.4; 4096 x 1024, group 64, M = 1 4.7.
+// Measured (us, weights from HBM, rates of codes and scales): 24576 x 4096, group 128, M = 16 20.0, 2.6 TB/s
+// (without the conversion about 15, the rest is the 192 tiles' uneven share of 148 SMs and 5 us of launch, fill and
+// merge); 4096 x 12288, group 32, M = 5 12.0, 2.4 TB/s; 6144 x 4096, M = 64 12.7; 4096 x 1024, group 64, M = 1 4.8.
 //
 // Unpacking is exact: a nibble q = code + 8 in the low mantissa bits of 128.0 is the bf16 number
 // 128 + q; subtracting 136 leaves the code. W itself is never rounded, x stays bf16.
@@ -22,10 +22,10 @@
 // and lost 15% at small sizes.) The packed layout keeps a block's codes and scales together, so a block is
 // one bulk copy (8 KB and 256 bytes a group) and two boxes of x. Warp roles: two sets of four unpacking warps
 // that take parts in turn, each with its A and D, a producer and an MMA warp, whose issue sits behind
-// elect.sync (behind `lane == 0` it took four times as long). Up to 32 rows two CTAs share an SM. The CTAs'
-// totals are pushed to the owner of each output through distributed shared memory and added in rank order:
-// one launch, no workspace, the same bits every time, and the result leaves finished (bf16, fp32
-// or SwiGLU).
+// elect.sync (behind `lane == 0` it took four times as long). Up to 32 rows two CTAs share an SM (but for 17 to 32
+// rows in groups of 32, whose A and D take 384 of the 512 tensor memory columns). The CTAs' totals are pushed to the
+// owner of each output through distributed shared memory and added in rank order: one launch, no workspace, the same
+// bits every time, and the result leaves finished (bf16, fp32 or SwiGLU).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -532,7 +532,10 @@ constexpr int kFixed = 8;
 // K splits: the least waves x (blocks of a CTA + what it costs beside them). Clusters that the device holds:
 // the occupancy query counts one CTA per SM for kernels with tensor memory. Two share an SM where kCtas is 2,
 // so a cluster of S also fits wherever one of S / 2 does with a CTA to an SM. At M = 16 it takes 8 for
-// 4096 x 12288 (11.9 us; 6: 13.9, 4: 16.5, 1: 47.6) and 1 for 24576 x 4096 (22.5; 2: 21.8, 4: 26.5, 8: 44.0).
+// 4096 x 12288 (11.5 us; 6: 12.7, 4: 14.9, 1: 42.1) and 1 for 24576 x 4096 (20.0; 2: 20.5, 4: 24.8, 8: 41.4); at
+// M = 64 2 for 6144 x 4096 (12.7; 1: 19.3, 4: 17.8). It does not count the merge, which grows with the cluster: 4
+// would be better than its 5 for 6144 x 4096 at M = 16 (7.9 against 8.8) and than its 8 for 4096 x 1024 at M = 1
+// (4.1 against 4.8).
 template <typename C>
 int launch(const CUtensorMap& xm, const Params& p, cudaStream_t stream) {
   const int blocks = p.layout.blocks(), tiles = p.layout.tiles;

@@ -27,9 +27,10 @@ from kernels.quant import Weight4
 
 #: Rows the skinny kernel takes (x is staged as 16/32/64-row slabs).
 MAX_ROWS = 64
-#: Rows that 4-bit weights take in launches of MAX_ROWS. 128 rows of [4096, 4096] in two: 17.9 us, expanded
-#: weights and cuBLAS 21.3 ([24576, 4096]: 71 and 125; [4096, 1024] loses 4 us); three launches of 192
-#: rows: 26.8 and 21.9.
+#: Rows that 4-bit weights take in launches of MAX_ROWS. 65 and 128 rows in two launches against expanded weights
+#: and cuBLAS, us: [4096, 4096] 16.0 and 18.5 against 22.8 and 23.0, [4096, 12288] 27 and 32 against 66, [24576, 4096] 57
+#: and 76 against 123 and 125, but [4096, 1024] 11.3 and 12.8 against 8.8. Three launches of 192 rows of
+#: [4096, 4096]: 26.8 against 21.9.
 MAX_ROWS4 = 2 * MAX_ROWS
 BF16_OUT, FP32_OUT, SWIGLU_OUT, SPLITS_OUT = 0, 1, 2, 3
 _SPLITS = {}
@@ -50,7 +51,8 @@ def keep_native(rows, weight):
     """engine/kernels/linear.py:484-486: leave ``rows`` x ``weight`` on cuBLAS without spending
     tuning time on it. The B200 projection has no timed search to skip, and the reference calls
     this only for row counts above MAX_ROWS (its verify blocks), which ``linear`` already routes
-    to cuBLAS; the shape is recorded so ``linear`` keeps it there whatever its row count."""
+    to cuBLAS; the shape is recorded so ``linear`` keeps it there whatever its row count. Products
+    with 4-bit weights keep their own rule: cuBLAS would need the weights expanded."""
     _NATIVE.add((weight.device, rows, weight.shape[0], weight.shape[1]))
 
 
